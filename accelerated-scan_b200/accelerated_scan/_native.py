@@ -44,6 +44,36 @@ class Plan(ctypes.Structure):
         return {name: getattr(self, name) for name, _ in self._fields_}
 
 
+_PTR, _I64, _I32 = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int32
+
+
+class Delta(ctypes.Structure):
+    """ascan_delta: the gated delta rule over whole sequences."""
+    _fields_ = ([(n, _PTR) for n in ("queries", "keys", "values", "log_gates", "betas")]
+                + [(n + "_stride", _I64 * 3) for n in ("queries", "keys", "values", "log_gates", "betas")]
+                + [("batch", _I64), ("seqlen", _I64)]
+                + [(n, _I32) for n in ("heads_k", "heads", "k_dim", "v_dim", "dtype", "log_gates_dtype", "betas_dtype")]
+                + [("scale", ctypes.c_float), ("initial_state", _PTR), ("seq_starts", _PTR), ("n_seqs", _I32),
+                   ("seq_starts_64", _I32)])
+
+
+class DeltaToken(ctypes.Structure):
+    """ascan_delta_token: one token of it for a batch of sequences."""
+    _fields_ = ([(n, _PTR) for n in ("queries", "keys", "values", "log_gates", "betas")]
+                + [(n + "_stride", _I64 * 2) for n in ("queries", "keys", "values", "log_gates", "betas")]
+                + [("batch", _I64)]
+                + [(n, _I32) for n in ("heads_k", "heads", "k_dim", "v_dim", "dtype", "log_gates_dtype", "betas_dtype")]
+                + [("scale", ctypes.c_float)])
+
+
+class Norm(ctypes.Structure):
+    """ascan_norm: norms around a block with its gate and residual scale."""
+    _fields_ = ([(n, _PTR) for n in ("x", "residual", "gate", "post_weight", "scale", "pre_weight")]
+                + [(n, _I64) for n in ("rows", "x_stride", "residual_stride", "gate_stride")]
+                + [(n, _I32) for n in ("dim", "dtype", "weights_dtype", "activation")]
+                + [("eps", ctypes.c_float), ("scale_value", ctypes.c_float)])
+
+
 def _load():
     if not os.path.exists(LIB_PATH):
         raise ImportError(
@@ -99,6 +129,23 @@ def _load():
     lib.ascan_peer_close.argtypes = [vp]
     lib.ascan_peer_free.restype = i32
     lib.ascan_peer_free.argtypes = [vp]
+    lib.ascan_delta_forward_bytes.restype = sz
+    lib.ascan_delta_forward_bytes.argtypes = [ctypes.POINTER(Delta), i32]
+    lib.ascan_delta_forward.restype = i32
+    lib.ascan_delta_forward.argtypes = [ctypes.POINTER(Delta), vp, vp, i32, vp, sz, vp]
+    lib.ascan_delta_backward_bytes.restype = sz
+    lib.ascan_delta_backward_bytes.argtypes = [ctypes.POINTER(Delta), vp, ctypes.POINTER(i64)]
+    lib.ascan_delta_backward.restype = i32
+    lib.ascan_delta_backward.argtypes = [ctypes.POINTER(Delta), vp, ctypes.POINTER(i64), vp, vp, vp, vp, vp, vp, vp, vp, sz,
+                                         vp, sz, vp]
+    lib.ascan_delta_step.restype = i32
+    lib.ascan_delta_step.argtypes = [ctypes.POINTER(DeltaToken), vp, vp, i64, i64, vp, i32, vp]
+    lib.ascan_norm_forward.restype = i32
+    lib.ascan_norm_forward.argtypes = [ctypes.POINTER(Norm), vp, vp, vp]
+    lib.ascan_norm_backward_bytes.restype = sz
+    lib.ascan_norm_backward_bytes.argtypes = [ctypes.POINTER(Norm)]
+    lib.ascan_norm_backward.restype = i32
+    lib.ascan_norm_backward.argtypes = [ctypes.POINTER(Norm), vp, i64, vp, i64, vp, vp, vp, vp, vp, vp, vp, sz, vp]
     lib.ascan_set_option.restype = i32
     lib.ascan_set_option.argtypes = [i32, i32]
     lib.ascan_get_option.restype = i32
@@ -115,6 +162,8 @@ EXPORTS = (
     "ascan_forward_sigmoid_gates", "ascan_backward_sigmoid_gates", "ascan_backward_complex_real_tokens",
     "ascan_check_no_alloc", "ascan_set_option", "ascan_get_option",
     "ascan_exchange_bytes", "ascan_workspace_bytes_time_sharded", "ascan_forward_time_sharded",
+    "ascan_delta_forward_bytes", "ascan_delta_forward", "ascan_delta_backward_bytes", "ascan_delta_backward",
+    "ascan_delta_step", "ascan_norm_forward", "ascan_norm_backward_bytes", "ascan_norm_backward",
     "ascan_backward_time_sharded", "ascan_peer_alloc", "ascan_peer_open", "ascan_peer_close", "ascan_peer_free",
 )
 
@@ -441,6 +490,119 @@ def backward_time_sharded(gates, states, grad_out, d_gates, d_tokens, rank: int,
                                              d_tokens.data_ptr(), rows, T, code, int(rank), int(world), int(call), table,
                                              _ptr(halo_state_left), ws.ptr, ws.nbytes, stream)
     _finish(rc, "ascan_backward_time_sharded", ws, stream)
+
+
+# Gated delta rule and norms.  Their kernels wait for nothing, keep nothing between calls and take ordinary tensors of
+# torch's allocator as scratch, so calls on different streams and captured graphs never share any.
+
+def _launched(rc, what, stream):
+    global launch_count
+    check(rc, what)
+    launch_count += 1
+    if _debug:
+        torch.cuda.ExternalStream(stream).synchronize() if stream else torch.cuda.synchronize()
+
+
+def delta_args(queries, keys, values, log_gates, betas, initial_state, scale, seq_starts) -> Delta:
+    """(B, T, heads, dim) tensors with a dense last dimension, in their own strides."""
+    a = Delta()
+    a.batch, a.seqlen, a.heads_k, a.k_dim = queries.shape
+    a.heads, a.v_dim = values.shape[2:]
+    for name, t in (("queries", queries), ("keys", keys), ("values", values), ("log_gates", log_gates), ("betas", betas)):
+        setattr(a, name, t.data_ptr())
+        setattr(a, name + "_stride", (_I64 * 3)(*t.stride()[:3]))
+    a.dtype, a.log_gates_dtype, a.betas_dtype = dtype_code(queries), dtype_code(log_gates), dtype_code(betas)
+    a.scale = scale
+    a.initial_state = _ptr(initial_state)
+    if seq_starts is not None:
+        a.seq_starts, a.n_seqs, a.seq_starts_64 = seq_starts.data_ptr(), seq_starts.numel() - 1, seq_starts.dtype == torch.int64
+    return a
+
+
+def delta_forward(a: Delta, device, out, final_state, keep: bool):
+    """Returns the scratch, which holds what `delta_backward` needs when keep."""
+    stream = _raw_stream(device)
+    with _device_guard(device):
+        nbytes = int(lib.ascan_delta_forward_bytes(ctypes.byref(a), int(keep)))
+        if nbytes == 0:
+            raise RuntimeError("delta: a shape that the kernels do not take (key dimension up to 128, value dimension up to 1024)")
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        rc = lib.ascan_delta_forward(ctypes.byref(a), out.data_ptr(), final_state.data_ptr(), int(keep), ws.data_ptr(), nbytes, stream)
+    _launched(rc, "ascan_delta_forward", stream)
+    return ws
+
+
+def delta_backward(a: Delta, device, d_out, d_final_state, grads, d_initial_state, kept):
+    """grads: tensors for the gradients of queries, keys, values, log_gates, betas."""
+    stream = _raw_stream(device)
+    strides = (_I64 * 3)(*d_out.stride()[:3])
+    with _device_guard(device):
+        nbytes = int(lib.ascan_delta_backward_bytes(ctypes.byref(a), d_out.data_ptr(), strides))
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        rc = lib.ascan_delta_backward(ctypes.byref(a), d_out.data_ptr(), strides, _ptr(d_final_state),
+                                      *(t.data_ptr() for t in grads), _ptr(d_initial_state), kept.data_ptr(), kept.numel(),
+                                      ws.data_ptr(), nbytes, stream)
+    _launched(rc, "ascan_delta_backward", stream)
+
+
+def delta_step(queries, keys, values, log_gates, betas, out, state, slots, scale):
+    a = DeltaToken()
+    a.batch, a.heads_k, a.k_dim = queries.shape
+    a.heads, a.v_dim = values.shape[1:]
+    for name, t in (("queries", queries), ("keys", keys), ("values", values), ("log_gates", log_gates), ("betas", betas)):
+        setattr(a, name, t.data_ptr())
+        setattr(a, name + "_stride", (_I64 * 2)(*t.stride()[:2]))
+    a.dtype, a.log_gates_dtype, a.betas_dtype = dtype_code(queries), dtype_code(log_gates), dtype_code(betas)
+    a.scale = scale
+    device = queries.device
+    stream = _raw_stream(device)
+    with _device_guard(device):
+        rc = lib.ascan_delta_step(ctypes.byref(a), out.data_ptr(), state.data_ptr(), state.shape[0], state.stride(0), _ptr(slots),
+                                  int(slots is not None and slots.dtype == torch.int64), stream)
+    _launched(rc, "ascan_delta_step", stream)
+
+
+def norm_args(x, residual, gate, post_weight, scale, pre_weight, activation: int, eps: float) -> Norm:
+    """(rows, dim) tensors with a dense last dimension; scale is a vector or a number."""
+    a = Norm()
+    a.rows, a.dim = x.shape
+    a.x, a.x_stride = x.data_ptr(), x.stride(0)
+    if residual is not None:
+        a.residual, a.residual_stride = residual.data_ptr(), residual.stride(0)
+    if gate is not None:
+        a.gate, a.gate_stride = gate.data_ptr(), gate.stride(0)
+    a.post_weight, a.pre_weight, a.scale_value = _ptr(post_weight), _ptr(pre_weight), 1.0
+    a.dtype = a.weights_dtype = dtype_code(x)
+    if isinstance(scale, torch.Tensor):
+        a.scale = scale.data_ptr()
+    else:
+        a.scale_value = scale
+    for w in (post_weight, pre_weight, scale):
+        if isinstance(w, torch.Tensor):
+            a.weights_dtype = dtype_code(w)
+    a.activation, a.eps = activation, eps
+    return a
+
+
+def norm_forward(a: Norm, device, hidden, normed):
+    stream = _raw_stream(device)
+    with _device_guard(device):
+        rc = lib.ascan_norm_forward(ctypes.byref(a), hidden.data_ptr(), _ptr(normed), stream)
+    _launched(rc, "ascan_norm_forward", stream)
+
+
+def norm_backward(a: Norm, device, d_hidden, d_normed, d_x, d_residual, d_gate, d_post_weight, d_scale, d_pre_weight):
+    stream = _raw_stream(device)
+    with _device_guard(device):
+        nbytes = 0
+        ws = None
+        if d_post_weight is not None or d_scale is not None or d_pre_weight is not None:
+            nbytes = int(lib.ascan_norm_backward_bytes(ctypes.byref(a)))
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        rc = lib.ascan_norm_backward(ctypes.byref(a), _ptr(d_hidden), 0 if d_hidden is None else d_hidden.stride(0), _ptr(d_normed),
+                                     0 if d_normed is None else d_normed.stride(0), d_x.data_ptr(), _ptr(d_residual), _ptr(d_gate),
+                                     _ptr(d_post_weight), _ptr(d_scale), _ptr(d_pre_weight), _ptr(ws), nbytes, stream)
+    _launched(rc, "ascan_norm_backward", stream)
 
 
 def exchange_bytes(rows: int, world: int) -> int:

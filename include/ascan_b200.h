@@ -342,6 +342,102 @@ int ascan_forward_no_alloc(const void *gates, const void *tokens, void *out,
  */
 int ascan_check_no_alloc(void *stream);
 
+/*
+ * Gated delta rule: a recurrence whose state is a k_dim x v_dim matrix per value head (fp32).  Per token
+ *     S' = exp(log_gate) S;   e = value - S'^T key;   S = S' + beta key e^T;   out = scale S^T query
+ * computed in chunks of 64 tokens.  No counterpart in the reference, whose state is one number per channel.
+ *   queries, keys   (batch, seqlen, heads_k, k_dim)     heads % heads_k == 0: value head h reads key head
+ *   values          (batch, seqlen, heads, v_dim)       h / (heads / heads_k)
+ *   log_gates, betas (batch, seqlen, heads)             of dtype, or float
+ * Strides are in elements, for batch, token and head; the last dimension is dense.  A log gate of -104 or less is
+ * a gate of zero.  initial_state (nullable) and final_state are dense (sequences, heads, k_dim, v_dim) floats, where
+ * sequences is batch, or n_seqs for a packed call: batch == 1 and sequence i holds the tokens seq_starts[i] ..
+ * seq_starts[i + 1] - 1 (n_seqs + 1 ascending int32, or int64 with seq_starts_64, on the device; sequences may be
+ * empty).  Tokens of a packed row that lie in no sequence get zeros in out and in every gradient.
+ * Limits: k_dim <= 128, v_dim <= 1024, heads <= 65535.
+ */
+typedef struct {
+    const void *queries, *keys, *values, *log_gates, *betas;
+    int64_t queries_stride[3], keys_stride[3], values_stride[3], log_gates_stride[3], betas_stride[3];
+    int64_t batch, seqlen;
+    int32_t heads_k, heads, k_dim, v_dim;
+    int32_t dtype, log_gates_dtype, betas_dtype;   /* ascan_dtype; ASCAN_C64 is refused       */
+    float scale;
+    const float *initial_state;
+    const void *seq_starts;
+    int32_t n_seqs, seq_starts_64;                 /* n_seqs == 0: not packed                 */
+} ascan_delta;
+
+/*
+ * Scratch bytes of ascan_delta_forward.  keep != 0: the scratch also receives what the backward reads (states at the
+ * chunks' starts, e of every token) and has to be handed to ascan_delta_backward unchanged.  0 for bad arguments.
+ */
+size_t ascan_delta_forward_bytes(const ascan_delta *args, int keep);
+
+/* out: dense (batch, seqlen, heads, v_dim) of dtype.  ws: 256-byte aligned, not initialised, one per call in flight. */
+int ascan_delta_forward(const ascan_delta *args, void *out, float *final_state, int keep,
+                        void *ws, size_t ws_bytes, void *stream);
+
+/* Scratch bytes of ascan_delta_backward for this gradient of out. */
+size_t ascan_delta_backward_bytes(const ascan_delta *args, const void *d_out, const int64_t *d_out_stride);
+
+/*
+ * Gradients of ascan_delta_forward, dense, of their inputs' shapes and types.  args and kept are those of a forward
+ * with keep != 0.  d_final_state may be NULL (zero), d_initial_state may be NULL (not wanted).  Heads that share a key
+ * head are summed in a fixed order.
+ */
+int ascan_delta_backward(const ascan_delta *args, const void *d_out, const int64_t *d_out_stride,
+                         const float *d_final_state, void *d_queries, void *d_keys, void *d_values,
+                         void *d_log_gates, void *d_betas, float *d_initial_state,
+                         void *kept, size_t kept_bytes, void *ws, size_t ws_bytes, void *stream);
+
+/*
+ * One token of the gated delta rule for a batch of sequences whose states lie in a pool, updated in place:
+ * state[slot] is a dense (heads, k_dim, v_dim) block of floats, slot_stride floats from slot to slot, pool slots.
+ * slots: `batch` int32 (int64 with slots_64), or NULL for slot b of row b.  A negative slot is a padded row: its out
+ * is zero.  A slot behind the pool, and one that an earlier row of the batch has, leave the pool alone and answer NaN.
+ * out: dense (batch, heads, v_dim).  Strides of the inputs: batch row and head.
+ */
+typedef struct {
+    const void *queries, *keys, *values, *log_gates, *betas;
+    int64_t queries_stride[2], keys_stride[2], values_stride[2], log_gates_stride[2], betas_stride[2];
+    int64_t batch;
+    int32_t heads_k, heads, k_dim, v_dim;
+    int32_t dtype, log_gates_dtype, betas_dtype;
+    float scale;
+} ascan_delta_token;
+int ascan_delta_step(const ascan_delta_token *args, void *out, float *state, int64_t pool, int64_t slot_stride,
+                     const void *slots, int slots_64, void *stream);
+
+/*
+ * Norms around a block with its gate and residual scale, rows of `dim` elements (at most 8192):
+ *     n = x rsqrt(mean(x^2) + eps) post_weight       (post_weight NULL: n = x)
+ *     hidden = residual + scale act(gate) n          (residual NULL: 0; gate NULL: act = 1)
+ *     normed = hidden rsqrt(mean(hidden^2) + eps) pre_weight       (pre_weight NULL: not computed)
+ * scale is a vector of dim elements, or scale_value where it is NULL.  activation: 0 the gate itself, 1 sigmoid,
+ * 2 z sigmoid(z).  The three vectors have weights_dtype: dtype or float.  Strides: elements from row to row.
+ * No counterpart in the reference.
+ */
+typedef struct {
+    const void *x, *residual, *gate, *post_weight, *scale, *pre_weight;
+    int64_t rows, x_stride, residual_stride, gate_stride;
+    int32_t dim, dtype, weights_dtype, activation;
+    float eps, scale_value;
+} ascan_norm;
+int ascan_norm_forward(const ascan_norm *args, void *hidden, void *normed, void *stream);
+
+/*
+ * Gradients: d_hidden and d_normed may be NULL (zero); d_residual, d_gate and the weights' may be NULL (not wanted).
+ * ws: ascan_norm_backward_bytes(args) bytes, 16-byte aligned, not initialised; only read where a weight's gradient is
+ * wanted.  Sums over rows run in a fixed order.
+ */
+size_t ascan_norm_backward_bytes(const ascan_norm *args);
+int ascan_norm_backward(const ascan_norm *args, const void *d_hidden, int64_t d_hidden_stride,
+                        const void *d_normed, int64_t d_normed_stride,
+                        void *d_x, void *d_residual, void *d_gate,
+                        void *d_post_weight, void *d_scale, void *d_pre_weight,
+                        void *ws, size_t ws_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
