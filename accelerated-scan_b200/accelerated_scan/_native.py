@@ -54,7 +54,7 @@ class Delta(ctypes.Structure):
                 + [("batch", _I64), ("seqlen", _I64)]
                 + [(n, _I32) for n in ("heads_k", "heads", "k_dim", "v_dim", "dtype", "log_gates_dtype", "betas_dtype")]
                 + [("scale", ctypes.c_float), ("initial_state", _PTR), ("seq_starts", _PTR), ("n_seqs", _I32),
-                   ("seq_starts_64", _I32)])
+                   ("seq_starts_64", _I32), ("status", _PTR)])
 
 
 class DeltaToken(ctypes.Structure):
@@ -500,7 +500,26 @@ def _launched(rc, what, stream):
     check(rc, what)
     launch_count += 1
     if _debug:
-        torch.cuda.ExternalStream(stream).synchronize() if stream else torch.cuda.synchronize()
+        torch.cuda.synchronize()
+        for index in list(_sinks):
+            _sink(torch.device("cuda", index))
+
+
+_sinks = {}
+
+
+def _sink(device):
+    """A word of pinned host memory per device, kept for good: a kernel whose bounded wait expires sets it, the next call
+    raises."""
+    sink = _sinks.get(device.index)
+    if sink is None:
+        word = torch.zeros(4, dtype=torch.int32).pin_memory()
+        sink = _sinks[device.index] = (word, word.numpy(), word.data_ptr())
+    if sink[1][0]:
+        sink[1][0] = 0
+        raise RuntimeError("accelerated_scan: a bounded device-side wait expired in an earlier launch on this device; its "
+                           "result is invalid (ascan status 4)")
+    return sink[2]
 
 
 def delta_args(queries, keys, values, log_gates, betas, initial_state, scale, seq_starts) -> Delta:
@@ -513,6 +532,7 @@ def delta_args(queries, keys, values, log_gates, betas, initial_state, scale, se
         setattr(a, name + "_stride", (_I64 * 3)(*t.stride()[:3]))
     a.dtype, a.log_gates_dtype, a.betas_dtype = dtype_code(queries), dtype_code(log_gates), dtype_code(betas)
     a.scale = scale
+    a.status = _sink(queries.device)
     a.initial_state = _ptr(initial_state)
     if seq_starts is not None:
         a.seq_starts, a.n_seqs, a.seq_starts_64 = seq_starts.data_ptr(), seq_starts.numel() - 1, seq_starts.dtype == torch.int64

@@ -41,10 +41,13 @@ static int check_shape(const ascan_delta *a) {
 
 static int terms(int dtype) { return dtype == ASCAN_BF16 ? 1 : 2; }
 
-// bf16 rows that the 16-byte copies can take as they are
-static bool is_plane(const void *p, const int64_t *s, int dtype, int d) {
-    if (dtype != ASCAN_BF16 || d % 8 != 0 || (reinterpret_cast<uintptr_t>(p) & 15)) return false;
-    return s[0] % 8 == 0 && s[1] % 8 == 0 && s[2] % 8 == 0;
+// bf16 rows that 16-byte copies and tensor maps can take as they are
+static bool is_plane(const ascan_delta *a, const void *p, const int64_t *s, int heads, int d) {
+    if (a->dtype != ASCAN_BF16 || d % 8 != 0 || (reinterpret_cast<uintptr_t>(p) & 15)) return false;
+    const int64_t sizes[3] = {a->batch, a->seqlen, heads};
+    for (int i = 0; i < 3; ++i)
+        if (s[i] % 8 != 0 || (sizes[i] > 1 && (s[i] <= 0 || s[i] >= int64_t(1) << 38))) return false;
+    return true;
 }
 
 struct Bump {          // 256-byte aligned pieces of one buffer
@@ -72,7 +75,7 @@ static Planes user_plane(const void *p, const int64_t *s) {
 
 static void plan_pack(const ascan_delta *a, const void *src, const int64_t *strides, int heads, int d, Planes *to, Bump &bump,
                       PackJob *jobs, int *n) {
-    if (is_plane(src, strides, a->dtype, d)) {
+    if (is_plane(a, src, strides, heads, d)) {
         *to = user_plane(src, strides);
         return;
     }
@@ -93,7 +96,14 @@ static int run_packs(const ascan_delta *a, const PackJob *jobs, int n, cudaStrea
     return ASCAN_OK;
 }
 
-static int fill(const ascan_delta *a, DeltaParams &p, Bump &bump, bool keep, PackJob *jobs, int *n_jobs) {
+static void take_chunks(DeltaParams &p, Bump &bump) {
+    const int64_t each = int64_t(p.slots) * p.H;
+    p.M = bump.take<__nv_bfloat16>(each * 2 * 4096);
+    p.P = bump.take<__nv_bfloat16>(each * 2 * 4096);
+}
+
+// keep: what the backward reads again comes first, so that the rest of the layout does not matter to it
+static void fill(const ascan_delta *a, DeltaParams &p, Bump &bump, bool keep, PackJob *jobs, int *n_jobs) {
     p.batch = a->batch;
     p.T = a->seqlen;
     p.packed = a->n_seqs > 0;
@@ -123,16 +133,16 @@ static int fill(const ascan_delta *a, DeltaParams &p, Bump &bump, bool keep, Pac
     plan_pack(a, a->keys, a->keys_stride, a->heads_k, a->k_dim, &p.k, bump, jobs, n_jobs);
     plan_pack(a, a->values, a->values_stride, a->heads, a->v_dim, &p.v, bump, jobs, n_jobs);
     const int64_t each = int64_t(p.slots) * p.H;
-    p.M = bump.take<__nv_bfloat16>(each * 2 * 4096);
-    p.P = bump.take<__nv_bfloat16>(each * 2 * 4096);
     p.sc = bump.take<float>(each * SC_ARRAYS * 64);
     if (keep) {
         const int nt = terms(a->dtype), kp = p.Kp <= 64 ? 64 : 128;
         p.S = bump.take<__nv_bfloat16>(each * nt * p.Vp * kp);
         p.e = bump.take<__nv_bfloat16>(each * nt * 64 * p.Vp);
     }
-    return ASCAN_OK;
+    p.status = a->status;
 }
+
+static bool tensor_core_path(const ascan_delta *a) { return a->dtype == ASCAN_BF16; }
 
 static void fill_back(const ascan_delta *a, DeltaParams &p, Bump &bump, const void *d_out, const int64_t *d_out_stride, PackJob *jobs,
                       int *n_jobs) {
@@ -140,6 +150,7 @@ static void fill_back(const ascan_delta *a, DeltaParams &p, Bump &bump, const vo
     const int nt = terms(a->dtype), kp = p.Kp <= 64 ? 64 : 128;
     p.dS = bump.take<__nv_bfloat16>(each * nt * p.Vp * kp);
     p.z = bump.take<__nv_bfloat16>(each * nt * 64 * p.Vp);
+    take_chunks(p, bump);
     plan_pack(a, d_out, d_out_stride, a->heads, a->v_dim, &p.d_out, bump, jobs, n_jobs);
 }
 
@@ -285,6 +296,7 @@ size_t ascan_delta_forward_bytes(const ascan_delta *a, int keep) {
     PackJob jobs[4];
     int n = 0;
     fill(a, p, bump, keep != 0, jobs, &n);
+    if (!tensor_core_path(a)) take_chunks(p, bump);
     return bump.used + 256;
 }
 
@@ -318,10 +330,12 @@ int ascan_delta_forward(const ascan_delta *a, void *out, float *final_state, int
     PackJob jobs[4];
     int n = 0;
     fill(a, p, bump, keep != 0, jobs, &n);
+    if (!tensor_core_path(a)) take_chunks(p, bump);
     p.out = out;
     p.s1 = final_state;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if ((rc = run_packs(a, jobs, n, st)) != ASCAN_OK) return rc;
+    if (tensor_core_path(a)) return delta_launch_sweep_tc(p, keep != 0, st);
     if ((rc = delta_launch_prep(p, terms(a->dtype), st)) != ASCAN_OK) return rc;
     return delta_launch_sweep(p, terms(a->dtype), keep != 0, sms, st);
 }
@@ -355,6 +369,7 @@ int ascan_delta_backward(const ascan_delta *a, const void *d_out, const int64_t 
     p.d_b = d_betas;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if ((rc = run_packs(a, jobs, n, st)) != ASCAN_OK) return rc;
+    if ((rc = delta_launch_prep(p, terms(a->dtype), st)) != ASCAN_OK) return rc;
     if ((rc = delta_launch_back_sweep(p, terms(a->dtype), sms, st)) != ASCAN_OK) return rc;
     return delta_launch_grads(p, terms(a->dtype), st);
 }

@@ -46,18 +46,20 @@ struct DeltaParams {
     // scratch
     __nv_bfloat16 *M, *P;            // [slot][H][2][64][64]
     float *sc;                       // [slot][H][SC_ARRAYS][64]
-    __nv_bfloat16 *S, *e;            // saved for the backward: [slot][H][nt][Vp][KP] and [slot][H][nt][64][Vp]
+    __nv_bfloat16 *S, *e;            // saved for the backward: [slot][H][nt][Vp][KP] and [slot][H][nt][Vp][64]
     // backward
     __nv_bfloat16 *dS, *z;           // as S and e
     const float *d_s1;
     float *d_s0;
     void *d_q, *d_k, *d_v, *d_g, *d_b;
+    int *status;                     // nullable, host memory: set when a bounded wait expired
 };
 
 int delta_launch_pack(const void *src, int dtype, const int64_t *strides, int64_t batch, int64_t T, int heads, int d,
                       int dp, __nv_bfloat16 *dst, int64_t plane, cudaStream_t st);
 int delta_launch_prep(const DeltaParams &p, int nt, cudaStream_t st);
 int delta_launch_sweep(const DeltaParams &p, int nt, bool save, int sm_count, cudaStream_t st);
+int delta_launch_sweep_tc(const DeltaParams &p, bool save, cudaStream_t st);
 int delta_launch_back_sweep(const DeltaParams &p, int nt, int sm_count, cudaStream_t st);
 int delta_launch_grads(const DeltaParams &p, int nt, cudaStream_t st);
 

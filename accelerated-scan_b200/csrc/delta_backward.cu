@@ -195,22 +195,29 @@ __global__ void __launch_bounds__(256, 1) delta_back_sweep_kernel(DeltaParams p)
                 mma(d[2 * np + 1], a[0], b[2], b[3]);
             }
         }
+        save_state<64, NT>(stg, stg_p, d, p.z + at * NT * 64 * p.Vp, v0, p.Vp, lane);
+        // y = beta z = dV
+#pragma unroll
+        for (int n = 0; n < 8; ++n) {
+            const float2 be = *reinterpret_cast<const float2 *>(sc + SC_BETA * 64 + 8 * n + t2);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) d[n][i] *= i & 1 ? be.y : be.x;
+        }
         stage_transposed<NT>(stg, stg_p, d, lane);
         __syncwarp();
-        flush_planes<NT>(stg_p, p.z + at * NT * 64 * p.Vp, v0, p.Vp, lane);
-        __syncwarp();
-        // dS -= K^T (gam beta z)
+        const int64_t tok = sq.t0 + int64_t(c) * 64, left = sq.len - int64_t(c) * 64;
+        flush_out<NT>(stg_p, p.d_v, p.dtype, ((sq.b * p.T + tok) * p.H + h) * int64_t(p.V), int64_t(p.H) * p.V,
+                      static_cast<int>(left < 64 ? left : 64), v0, p.V, lane);
+        // dS -= K^T (gam y)
 #pragma unroll
         for (int kk = 0; kk < 4; ++kk) {
             uint32_t as[2][4];
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-                const float2 be = *reinterpret_cast<const float2 *>(sc + SC_BETA * 64 + 16 * kk + 8 * j + t2);
                 const float2 ga = *reinterpret_cast<const float2 *>(sc + SC_GAM * 64 + 16 * kk + 8 * j + t2);
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
-                    split2(-ga.x * be.x * d[2 * kk + j][2 * i], -ga.y * be.y * d[2 * kk + j][2 * i + 1], as[0][2 * j + i],
-                           as[1][2 * j + i]);
+                    split2(-ga.x * d[2 * kk + j][2 * i], -ga.y * d[2 * kk + j][2 * i + 1], as[0][2 * j + i], as[1][2 * j + i]);
             }
 #pragma unroll
             for (int np = 0; np < KP / 16; ++np) {
@@ -273,8 +280,8 @@ struct GradLayout {
     static constexpr int TOK = 64 * VS * 2, STATE = VS * KP * 2;
     static constexpr int SLAB = NT * (3 * TOK + 2 * STATE);
     static constexpr int K = 0, Q = NT * TILE, D = 2 * NT * TILE, F = D + NT * 8192, SLABS = F + NT * 8192;
-    static constexpr int SC = SLABS + 2 * SLAB, RED = SC + SC_ARRAYS * 256, BYTES = RED + 1024 + 64;
-    // inside a slab
+    static constexpr int SC = SLABS + 2 * SLAB, RED = SC + SC_ARRAYS * 256, BYTES = RED + (192 + 256) * 4;
+    // inside a slab; e and z lie transposed, VS rows of 64 tokens
     static constexpr int DO = 0, E = NT * TOK, Z = 2 * NT * TOK, S = 3 * NT * TOK, DS = S + NT * STATE;
 };
 
@@ -286,8 +293,8 @@ __device__ __forceinline__ void grad_load(const DeltaParams &p, uint32_t base, c
     for (int pl = 0; pl < NT; ++pl) {
         load_tile<L::VCH>(base + L::DO + pl * L::TOK, p.d_out.p + pl * p.d_out.plane + ch.b * p.d_out.sb + ch.t0 * p.d_out.st +
                           h * p.d_out.sh + v0, p.d_out.st, ch.rows, pieces, tid, 256);
-        load_tile<L::VCH>(base + L::E + pl * L::TOK, p.e + (at * NT + pl) * 64 * p.Vp + v0, p.Vp, 64, pieces, tid, 256);
-        load_tile<L::VCH>(base + L::Z + pl * L::TOK, p.z + (at * NT + pl) * 64 * p.Vp + v0, p.Vp, 64, pieces, tid, 256);
+        load_tile<8>(base + L::E + pl * L::TOK, p.e + ((at * NT + pl) * p.Vp + v0) * 64, 64, rows, 8, tid, 256, L::VS);
+        load_tile<8>(base + L::Z + pl * L::TOK, p.z + ((at * NT + pl) * p.Vp + v0) * 64, 64, rows, 8, tid, 256, L::VS);
         load_tile<KP / 8>(base + L::S + pl * L::STATE, p.S + ((at * NT + pl) * p.Vp + v0) * KP, KP, rows, KP / 8, tid, 256, L::VS);
         load_tile<KP / 8>(base + L::DS + pl * L::STATE, p.dS + ((at * NT + pl) * p.Vp + v0) * KP, KP, rows, KP / 8, tid, 256, L::VS);
     }
@@ -415,8 +422,8 @@ __global__ void __launch_bounds__(256, 1) delta_grads_kernel(DeltaParams p) {
 #pragma unroll
             for (int pl = 0; pl < NT; ++pl) {
                 ldsm4(ao[pl], addr_an<L::VCH>(sb + L::DO + pl * L::TOK, 16 * wr, 2 * kk, lane));
-                ldsm4(ae[pl], addr_an<L::VCH>(sb + L::E + pl * L::TOK, 16 * wr, 2 * kk, lane));
-                ldsm4(az[pl], addr_an<L::VCH>(sb + L::Z + pl * L::TOK, 16 * wr, 2 * kk, lane));
+                ldsm4t(ae[pl], addr_at<8>(sb + L::E + pl * L::TOK, 16 * kk, 2 * wr, lane));
+                ldsm4t(az[pl], addr_at<8>(sb + L::Z + pl * L::TOK, 16 * kk, 2 * wr, lane));
             }
 #pragma unroll
             for (int np = 0; np < KT / 2; ++np)
@@ -444,7 +451,7 @@ __global__ void __launch_bounds__(256, 1) delta_grads_kernel(DeltaParams p) {
 #pragma unroll
                 for (int pl = 0; pl < NT; ++pl) {
                     uint32_t b[4];
-                    ldsm4(b, addr_bn<L::VCH>(sb + L::E + pl * L::TOK, 32 * wc + 16 * np, 2 * kk, lane));
+                    ldsm4t(b, addr_bt<8>(sb + L::E + pl * L::TOK, 16 * kk, 4 * wc + 2 * np, lane));
 #pragma unroll
                     for (int pa = 0; pa + pl < NT; ++pa) {
                         mma(dp[2 * np], ao[pa], b[0], b[1]);
@@ -455,23 +462,17 @@ __global__ void __launch_bounds__(256, 1) delta_grads_kernel(DeltaParams p) {
                 }
             }
         }
-        {   // dbeta = e . z and dV = beta z: four threads a token;  <S0, dS1>: every thread
-            const int t = tid >> 2;
-            const float be = ssc[SC_BETA * 64 + t];
-#pragma unroll
-            for (int i = 0; i < L::VCH / 4; ++i) {
-                const int pc = (tid & 3) + 4 * i, v = v0 + pc * 8;
-                if (v >= p.Vp) continue;
-                float e[8], z[8];
-                read8<NT>(sp + L::E, L::TOK, tile_off<L::VCH>(t, pc), e);
-                read8<NT>(sp + L::Z, L::TOK, tile_off<L::VCH>(t, pc), z);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) dbeta += e[j] * z[j];
-                if (t < ch.rows) {
-                    const int64_t o = ((ch.b * p.T + ch.t0 + t) * p.H + h) * p.V;
-#pragma unroll
-                    for (int j = 0; j < 8; j += 2) store_pair(p.d_v, p.dtype, o, v + j, p.V, be * z[j], be * z[j + 1], p.V % 2 == 0);
+        {   // dbeta = e . z: four threads a token, a quarter of the slab each;  <S0, dS1>: every thread
+            const int t = tid & 63, part = tid >> 6;
+            for (int i = 0; i < L::VS / 4; ++i) {
+                const uint32_t o = tile_off<8>(part * (L::VS / 4) + i, t >> 3) + (t & 7) * 2;
+                float e = __bfloat162float(*reinterpret_cast<const bf16 *>(sp + L::E + o));
+                float z = __bfloat162float(*reinterpret_cast<const bf16 *>(sp + L::Z + o));
+                if (NT == 2) {
+                    e += __bfloat162float(*reinterpret_cast<const bf16 *>(sp + L::E + L::TOK + o));
+                    z += __bfloat162float(*reinterpret_cast<const bf16 *>(sp + L::Z + L::TOK + o));
                 }
+                dbeta += e * z;
             }
             for (int i = tid; i < L::VS * NCH; i += 256) {
                 float a[8], b[8];
@@ -571,11 +572,13 @@ __global__ void __launch_bounds__(256, 1) delta_grads_kernel(DeltaParams p) {
 #pragma unroll
             for (int d = 16; d; d /= 2) dot_s += __shfl_xor_sync(~0u, dot_s, d);
             if (lane == 0) red[128 + warp] = dot_s;
-            dbeta += __shfl_xor_sync(~0u, dbeta, 1);
-            dbeta += __shfl_xor_sync(~0u, dbeta, 2);
+            red[192 + tid] = dbeta;
             const int64_t row = ch.b * p.T + ch.t0;
-            if ((tid & 3) == 0 && (tid >> 2) < ch.rows) store_from_float(p.d_b, p.b_dtype, (row + (tid >> 2)) * p.H + h, dbeta);
             __syncthreads();
+            if (tid >= 64 && tid - 64 < ch.rows) {
+                const float *r = red + 128 + tid;
+                store_from_float(p.d_b, p.b_dtype, (row + tid - 64) * p.H + h, (r[0] + r[64]) + (r[128] + r[192]));
+            }
             if (warp == 0) {            // sums of dG from each token to the end; the state's share stands on the last one
                 float x[2], tail = 0.f;
 #pragma unroll

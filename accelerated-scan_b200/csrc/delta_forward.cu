@@ -449,12 +449,7 @@ __global__ void __launch_bounds__(256, 1) delta_sweep_kernel(DeltaParams p) {
                 mma(x[2 * np + 1], a[0], b[2], b[3]);
             }
         }
-        if (SAVE) {
-            stage_transposed<NT>(stg, stg_p, x, lane);
-            __syncwarp();
-            flush_planes<NT>(stg_p, p.e + at * NT * 64 * p.Vp, v0, p.Vp, lane);
-            __syncwarp();
-        }
+        if (SAVE) save_state<64, NT>(stg, stg_p, x, p.e + at * NT * 64 * p.Vp, v0, p.Vp, lane);
         const float gam_c = sc[SC_GAM * 64 + 63];
 #pragma unroll
         for (int n = 0; n < KT; ++n)

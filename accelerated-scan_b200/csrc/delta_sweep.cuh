@@ -53,30 +53,8 @@ __device__ __forceinline__ void flush_out(const unsigned char *stg, void *dst, i
     }
 }
 
-// ... to bf16 planes [plane][64][Vp]
-template <int NT>
-__device__ __forceinline__ void flush_planes(const unsigned char *stg, bf16 *dst, int v0, int Vp, int lane) {
-    for (int i = lane; i < 128; i += 32) {
-        const int t = i >> 1, pc = i & 1, v = v0 + pc * 8;
-        if (v >= Vp) continue;
-        if (NT == 1) {
-            *reinterpret_cast<uint4 *>(dst + t * Vp + v) = *reinterpret_cast<const uint4 *>(stg + (pc * 64 + t) * 16);
-        } else {
-            const float *f = reinterpret_cast<const float *>(stg);
-            const float4 a = *reinterpret_cast<const float4 *>(f + ((2 * pc) * 64 + t) * 4);
-            const float4 b = *reinterpret_cast<const float4 *>(f + ((2 * pc + 1) * 64 + t) * 4);
-            uint4 hi, lo;
-            split2(a.x, a.y, hi.x, lo.x);
-            split2(a.z, a.w, hi.y, lo.y);
-            split2(b.x, b.y, hi.z, lo.z);
-            split2(b.z, b.w, hi.w, lo.w);
-            *reinterpret_cast<uint4 *>(dst + t * Vp + v) = hi;
-            *reinterpret_cast<uint4 *>(dst + 64 * Vp + t * Vp + v) = lo;
-        }
-    }
-}
-
-// the warp's 16 x K accumulators to bf16 planes [plane][Vp][KP], through the staging area
+// the warp's 16 x KP accumulators (of the state, or KP = 64 tokens of e or z) to bf16 planes [plane][Vp][KP], through the
+// staging area
 template <int KP, int NT>
 __device__ __forceinline__ void save_state(uint32_t stg, const unsigned char *stg_p, const float (&s)[KP / 8][4], bf16 *dst, int v0,
                                            int Vp, int lane) {

@@ -366,6 +366,8 @@ typedef struct {
     const float *initial_state;
     const void *seq_starts;
     int32_t n_seqs, seq_starts_64;                 /* n_seqs == 0: not packed                 */
+    int *status;                                   /* nullable, device-accessible host memory: a kernel whose bounded
+                                                      wait expired stores 1; its results are then invalid */
 } ascan_delta;
 
 /*

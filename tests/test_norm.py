@@ -11,6 +11,11 @@ from accelerated_scan import norm
 SUMS = 16 * 2.0 ** -24
 
 
+@pytest.fixture(autouse=True)
+def seeded():
+    torch.manual_seed(0)
+
+
 def tol(dtype):
     return torch.finfo(dtype).eps / 2 + SUMS
 
