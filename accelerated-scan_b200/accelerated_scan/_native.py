@@ -10,6 +10,7 @@ from __future__ import annotations
 import contextlib
 import ctypes
 import os
+import struct
 
 import torch
 
@@ -63,7 +64,7 @@ class DeltaToken(ctypes.Structure):
                 + [(n + "_stride", _I64 * 2) for n in ("queries", "keys", "values", "log_gates", "betas")]
                 + [("batch", _I64)]
                 + [(n, _I32) for n in ("heads_k", "heads", "k_dim", "v_dim", "dtype", "log_gates_dtype", "betas_dtype")]
-                + [("scale", ctypes.c_float)])
+                + [("scale", ctypes.c_float), ("status", _PTR)])
 
 
 class Norm(ctypes.Structure):
@@ -71,7 +72,7 @@ class Norm(ctypes.Structure):
     _fields_ = ([(n, _PTR) for n in ("x", "residual", "gate", "post_weight", "scale", "pre_weight")]
                 + [(n, _I64) for n in ("rows", "x_stride", "residual_stride", "gate_stride")]
                 + [(n, _I32) for n in ("dim", "dtype", "weights_dtype", "activation")]
-                + [("eps", ctypes.c_float), ("scale_value", ctypes.c_float)])
+                + [("eps", ctypes.c_float), ("scale_value", ctypes.c_float), ("status", _PTR)])
 
 
 def _load():
@@ -130,22 +131,22 @@ def _load():
     lib.ascan_peer_free.restype = i32
     lib.ascan_peer_free.argtypes = [vp]
     lib.ascan_delta_forward_bytes.restype = sz
-    lib.ascan_delta_forward_bytes.argtypes = [ctypes.POINTER(Delta), i32]
+    lib.ascan_delta_forward_bytes.argtypes = [vp, i32]
     lib.ascan_delta_forward.restype = i32
-    lib.ascan_delta_forward.argtypes = [ctypes.POINTER(Delta), vp, vp, i32, vp, sz, vp]
+    lib.ascan_delta_forward.argtypes = [vp, vp, vp, i32, vp, sz, vp]
     lib.ascan_delta_backward_bytes.restype = sz
-    lib.ascan_delta_backward_bytes.argtypes = [ctypes.POINTER(Delta), vp, ctypes.POINTER(i64)]
+    lib.ascan_delta_backward_bytes.argtypes = [vp, vp, vp]
     lib.ascan_delta_backward.restype = i32
-    lib.ascan_delta_backward.argtypes = [ctypes.POINTER(Delta), vp, ctypes.POINTER(i64), vp, vp, vp, vp, vp, vp, vp, vp, sz,
+    lib.ascan_delta_backward.argtypes = [vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, sz,
                                          vp, sz, vp]
     lib.ascan_delta_step.restype = i32
-    lib.ascan_delta_step.argtypes = [ctypes.POINTER(DeltaToken), vp, vp, i64, i64, vp, i32, vp]
+    lib.ascan_delta_step.argtypes = [vp, vp, vp, i64, i64, vp, i32, vp]
     lib.ascan_norm_forward.restype = i32
-    lib.ascan_norm_forward.argtypes = [ctypes.POINTER(Norm), vp, vp, vp]
+    lib.ascan_norm_forward.argtypes = [vp, vp, vp, vp]
     lib.ascan_norm_backward_bytes.restype = sz
-    lib.ascan_norm_backward_bytes.argtypes = [ctypes.POINTER(Norm)]
+    lib.ascan_norm_backward_bytes.argtypes = [vp]
     lib.ascan_norm_backward.restype = i32
-    lib.ascan_norm_backward.argtypes = [ctypes.POINTER(Norm), vp, i64, vp, i64, vp, vp, vp, vp, vp, vp, vp, sz, vp]
+    lib.ascan_norm_backward.argtypes = [vp, vp, i64, vp, i64, vp, vp, vp, vp, vp, vp, vp, sz, vp]
     lib.ascan_set_option.restype = i32
     lib.ascan_set_option.argtypes = [i32, i32]
     lib.ascan_get_option.restype = i32
@@ -495,7 +496,7 @@ def backward_time_sharded(gates, states, grad_out, d_gates, d_tokens, rank: int,
 # Gated delta rule and norms.  Their kernels wait for nothing, keep nothing between calls and take ordinary tensors of
 # torch's allocator as scratch, so calls on different streams and captured graphs never share any.
 
-def _launched(rc, what, stream):
+def _launched(rc, what):
     global launch_count
     check(rc, what)
     launch_count += 1
@@ -522,107 +523,97 @@ def _sink(device):
     return sink[2]
 
 
-def delta_args(queries, keys, values, log_gates, betas, initial_state, scale, seq_starts) -> Delta:
-    """(B, T, heads, dim) tensors with a dense last dimension, in their own strides."""
-    a = Delta()
-    a.batch, a.seqlen, a.heads_k, a.k_dim = queries.shape
-    a.heads, a.v_dim = values.shape[2:]
-    for name, t in (("queries", queries), ("keys", keys), ("values", values), ("log_gates", log_gates), ("betas", betas)):
-        setattr(a, name, t.data_ptr())
-        setattr(a, name + "_stride", (_I64 * 3)(*t.stride()[:3]))
-    a.dtype, a.log_gates_dtype, a.betas_dtype = dtype_code(queries), dtype_code(log_gates), dtype_code(betas)
-    a.scale = scale
-    a.status = _sink(queries.device)
-    a.initial_state = _ptr(initial_state)
-    if seq_starts is not None:
-        a.seq_starts, a.n_seqs, a.seq_starts_64 = seq_starts.data_ptr(), seq_starts.numel() - 1, seq_starts.dtype == torch.int64
-    return a
+# The argument structures as bytes: one packing call costs a tenth of filling a ctypes.Structure field by field.
+_DELTA = struct.Struct("@5P15q2q7ifPPiiP")
+_TOKEN = struct.Struct("@5P10qq7ifP")
+_NORM = struct.Struct("@6P4q4i2fP")
+_STRIDES = struct.Struct("@3q")
+assert (_DELTA.size, _TOKEN.size, _NORM.size) == tuple(map(ctypes.sizeof, (Delta, DeltaToken, Norm)))
 
 
-def delta_forward(a: Delta, device, out, final_state, keep: bool):
+def delta_args(queries, keys, values, log_gates, betas, initial_state, scale, seq_starts) -> bytes:
+    """ascan_delta of (B, T, heads, dim) tensors with a dense last dimension, in their own strides."""
+    B, T, heads_k, K = queries.shape
+    _, _, heads, V = values.shape
+    packed = seq_starts is not None
+    return _DELTA.pack(
+        queries.data_ptr(), keys.data_ptr(), values.data_ptr(), log_gates.data_ptr(), betas.data_ptr(),
+        *queries.stride()[:3], *keys.stride()[:3], *values.stride()[:3], *log_gates.stride(), *betas.stride(),
+        B, T, heads_k, heads, K, V, DTYPE_CODE[queries.dtype], DTYPE_CODE[log_gates.dtype], DTYPE_CODE[betas.dtype], scale,
+        0 if initial_state is None else initial_state.data_ptr(), seq_starts.data_ptr() if packed else 0,
+        seq_starts.shape[0] - 1 if packed else 0, packed and seq_starts.dtype == torch.int64, _sink(queries.device))
+
+
+def delta_forward(args: bytes, device, out, final_state, keep: bool):
     """Returns the scratch, which holds what `delta_backward` needs when keep."""
     stream = _raw_stream(device)
     with _device_guard(device):
-        nbytes = int(lib.ascan_delta_forward_bytes(ctypes.byref(a), int(keep)))
+        nbytes = lib.ascan_delta_forward_bytes(args, keep)
         if nbytes == 0:
             raise RuntimeError("delta: a shape that the kernels do not take (key dimension up to 128, value dimension up to 1024)")
         ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
-        rc = lib.ascan_delta_forward(ctypes.byref(a), out.data_ptr(), final_state.data_ptr(), int(keep), ws.data_ptr(), nbytes, stream)
-    _launched(rc, "ascan_delta_forward", stream)
+        rc = lib.ascan_delta_forward(args, out.data_ptr(), final_state.data_ptr(), keep, ws.data_ptr(), nbytes, stream)
+    _launched(rc, "ascan_delta_forward")
     return ws
 
 
-def delta_backward(a: Delta, device, d_out, d_final_state, grads, d_initial_state, kept):
+def delta_backward(args: bytes, device, d_out, d_final_state, grads, d_initial_state, kept):
     """grads: tensors for the gradients of queries, keys, values, log_gates, betas."""
     stream = _raw_stream(device)
-    strides = (_I64 * 3)(*d_out.stride()[:3])
+    strides = _STRIDES.pack(*d_out.stride()[:3])
     with _device_guard(device):
-        nbytes = int(lib.ascan_delta_backward_bytes(ctypes.byref(a), d_out.data_ptr(), strides))
+        nbytes = lib.ascan_delta_backward_bytes(args, d_out.data_ptr(), strides)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
-        rc = lib.ascan_delta_backward(ctypes.byref(a), d_out.data_ptr(), strides, _ptr(d_final_state),
-                                      *(t.data_ptr() for t in grads), _ptr(d_initial_state), kept.data_ptr(), kept.numel(),
-                                      ws.data_ptr(), nbytes, stream)
-    _launched(rc, "ascan_delta_backward", stream)
+        rc = lib.ascan_delta_backward(args, d_out.data_ptr(), strides, _ptr(d_final_state), *[t.data_ptr() for t in grads],
+                                      _ptr(d_initial_state), kept.data_ptr(), kept.numel(), ws.data_ptr(), nbytes, stream)
+    _launched(rc, "ascan_delta_backward")
 
 
 def delta_step(queries, keys, values, log_gates, betas, out, state, slots, scale):
-    a = DeltaToken()
-    a.batch, a.heads_k, a.k_dim = queries.shape
-    a.heads, a.v_dim = values.shape[1:]
-    for name, t in (("queries", queries), ("keys", keys), ("values", values), ("log_gates", log_gates), ("betas", betas)):
-        setattr(a, name, t.data_ptr())
-        setattr(a, name + "_stride", (_I64 * 2)(*t.stride()[:2]))
-    a.dtype, a.log_gates_dtype, a.betas_dtype = dtype_code(queries), dtype_code(log_gates), dtype_code(betas)
-    a.scale = scale
+    B, heads_k, K = queries.shape
+    _, heads, V = values.shape
+    args = _TOKEN.pack(
+        queries.data_ptr(), keys.data_ptr(), values.data_ptr(), log_gates.data_ptr(), betas.data_ptr(),
+        *queries.stride()[:2], *keys.stride()[:2], *values.stride()[:2], *log_gates.stride(), *betas.stride(),
+        B, heads_k, heads, K, V, DTYPE_CODE[queries.dtype], DTYPE_CODE[log_gates.dtype], DTYPE_CODE[betas.dtype], scale,
+        _sink(queries.device))
     device = queries.device
-    stream = _raw_stream(device)
     with _device_guard(device):
-        rc = lib.ascan_delta_step(ctypes.byref(a), out.data_ptr(), state.data_ptr(), state.shape[0], state.stride(0), _ptr(slots),
-                                  int(slots is not None and slots.dtype == torch.int64), stream)
-    _launched(rc, "ascan_delta_step", stream)
+        rc = lib.ascan_delta_step(args, out.data_ptr(), state.data_ptr(), state.shape[0], state.stride(0), _ptr(slots),
+                                  slots is not None and slots.dtype == torch.int64, _raw_stream(device))
+    _launched(rc, "ascan_delta_step")
 
 
-def norm_args(x, residual, gate, post_weight, scale, pre_weight, activation: int, eps: float) -> Norm:
-    """(rows, dim) tensors with a dense last dimension; scale is a vector or a number."""
-    a = Norm()
-    a.rows, a.dim = x.shape
-    a.x, a.x_stride = x.data_ptr(), x.stride(0)
-    if residual is not None:
-        a.residual, a.residual_stride = residual.data_ptr(), residual.stride(0)
-    if gate is not None:
-        a.gate, a.gate_stride = gate.data_ptr(), gate.stride(0)
-    a.post_weight, a.pre_weight, a.scale_value = _ptr(post_weight), _ptr(pre_weight), 1.0
-    a.dtype = a.weights_dtype = dtype_code(x)
-    if isinstance(scale, torch.Tensor):
-        a.scale = scale.data_ptr()
-    else:
-        a.scale_value = scale
-    for w in (post_weight, pre_weight, scale):
-        if isinstance(w, torch.Tensor):
-            a.weights_dtype = dtype_code(w)
-    a.activation, a.eps = activation, eps
-    return a
+def norm_args(x, residual, gate, post_weight, scale, pre_weight, activation: int, eps: float) -> bytes:
+    """ascan_norm of (rows, dim) tensors with a dense last dimension; scale is a vector or a number."""
+    vector = isinstance(scale, torch.Tensor)
+    weights = post_weight if post_weight is not None else pre_weight if pre_weight is not None else scale if vector else x
+    return _NORM.pack(
+        x.data_ptr(), 0 if residual is None else residual.data_ptr(), 0 if gate is None else gate.data_ptr(),
+        0 if post_weight is None else post_weight.data_ptr(), scale.data_ptr() if vector else 0,
+        0 if pre_weight is None else pre_weight.data_ptr(),
+        x.shape[0], x.stride(0), 0 if residual is None else residual.stride(0), 0 if gate is None else gate.stride(0),
+        x.shape[1], DTYPE_CODE[x.dtype], DTYPE_CODE[weights.dtype], activation, eps, 1.0 if vector else scale,
+        _sink(x.device))
 
 
-def norm_forward(a: Norm, device, hidden, normed):
-    stream = _raw_stream(device)
+def norm_forward(args: bytes, device, hidden, normed):
     with _device_guard(device):
-        rc = lib.ascan_norm_forward(ctypes.byref(a), hidden.data_ptr(), _ptr(normed), stream)
-    _launched(rc, "ascan_norm_forward", stream)
+        rc = lib.ascan_norm_forward(args, hidden.data_ptr(), _ptr(normed), _raw_stream(device))
+    _launched(rc, "ascan_norm_forward")
 
 
-def norm_backward(a: Norm, device, d_hidden, d_normed, d_x, d_residual, d_gate, d_post_weight, d_scale, d_pre_weight):
-    stream = _raw_stream(device)
+def norm_backward(args: bytes, device, d_hidden, d_normed, d_x, d_residual, d_gate, d_post_weight, d_scale, d_pre_weight):
     with _device_guard(device):
         nbytes = 0
         ws = None
         if d_post_weight is not None or d_scale is not None or d_pre_weight is not None:
-            nbytes = int(lib.ascan_norm_backward_bytes(ctypes.byref(a)))
+            nbytes = lib.ascan_norm_backward_bytes(args)
             ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
-        rc = lib.ascan_norm_backward(ctypes.byref(a), _ptr(d_hidden), 0 if d_hidden is None else d_hidden.stride(0), _ptr(d_normed),
+        rc = lib.ascan_norm_backward(args, _ptr(d_hidden), 0 if d_hidden is None else d_hidden.stride(0), _ptr(d_normed),
                                      0 if d_normed is None else d_normed.stride(0), d_x.data_ptr(), _ptr(d_residual), _ptr(d_gate),
-                                     _ptr(d_post_weight), _ptr(d_scale), _ptr(d_pre_weight), _ptr(ws), nbytes, stream)
-    _launched(rc, "ascan_norm_backward", stream)
+                                     _ptr(d_post_weight), _ptr(d_scale), _ptr(d_pre_weight), _ptr(ws), nbytes, _raw_stream(device))
+    _launched(rc, "ascan_norm_backward")
 
 
 def exchange_bytes(rows: int, world: int) -> int:

@@ -38,17 +38,15 @@ def _check_inputs(lead, queries, keys, values, log_gates, betas):
         raise RuntimeError(f"key dimension {K} and value dimension {V}: expected 1 to {MAX_KEY_DIM} and 1 to {MAX_VALUE_DIM}")
     if queries.dtype not in _DTYPES:
         raise RuntimeError(f"unsupported dtype {queries.dtype}: expected float32, bfloat16 or float16")
-    for t in (keys, values):
-        if t.dtype != queries.dtype:
-            raise RuntimeError("queries, keys and values must have the same dtype")
-    for t in (log_gates, betas):
-        if t.dtype not in (queries.dtype, torch.float32):
-            raise RuntimeError("log_gates and betas must be float32 or of the queries' dtype")
-    for t in (queries, keys, values, log_gates, betas):
-        if not t.is_cuda:
-            raise RuntimeError("tensors must be CUDA tensors")
-        if t.device != queries.device:
-            raise RuntimeError("all tensors must be on the same device")
+    dtype, device = queries.dtype, queries.device
+    if keys.dtype != dtype or values.dtype != dtype:
+        raise RuntimeError("queries, keys and values must have the same dtype")
+    if log_gates.dtype not in (dtype, torch.float32) or betas.dtype not in (dtype, torch.float32):
+        raise RuntimeError("log_gates and betas must be float32 or of the queries' dtype")
+    if not queries.is_cuda:
+        raise RuntimeError("tensors must be CUDA tensors")
+    if keys.device != device or values.device != device or log_gates.device != device or betas.device != device:
+        raise RuntimeError("all tensors must be on the same device")
 
 
 def _dense_last(t):
@@ -56,25 +54,28 @@ def _dense_last(t):
     return t if t.shape[-1] <= 1 or t.stride(-1) == 1 else t.contiguous()
 
 
+def _forward(queries, keys, values, log_gates, betas, initial_state, scale, seq_starts, keep):
+    B, T, _, K = queries.shape
+    H, V = values.shape[2:]
+    n = B if seq_starts is None else seq_starts.shape[0] - 1
+    out = torch.empty(B, T, H, V, dtype=values.dtype, device=values.device)
+    state = torch.empty(n, H, K, V, dtype=torch.float32, device=values.device)
+    kept = None
+    if n:
+        args = _native.delta_args(queries, keys, values, log_gates, betas, initial_state, scale, seq_starts)
+        kept = _native.delta_forward(args, values.device, out, state, keep)
+    return out, state, kept
+
+
 class DeltaScan(torch.autograd.Function):
     @staticmethod
     def forward(ctx, queries, keys, values, log_gates, betas, initial_state, scale, seq_starts):
         queries, keys, values = _dense_last(queries), _dense_last(keys), _dense_last(values)
-        B, T, _, K = queries.shape
-        H, V = values.shape[2:]
-        n = B if seq_starts is None else seq_starts.numel() - 1
         s0 = None if initial_state is None else initial_state.float().contiguous()
-        out = torch.empty(B, T, H, V, dtype=values.dtype, device=values.device)
-        state = torch.empty(n, H, K, V, dtype=torch.float32, device=values.device)
-        keep = any(ctx.needs_input_grad[:6])
-        kept = None
-        if n:
-            args = _native.delta_args(queries, keys, values, log_gates, betas, s0, scale, seq_starts)
-            kept = _native.delta_forward(args, values.device, out, state, keep)
-        if keep:
-            ctx.save_for_backward(queries, keys, values, log_gates, betas, s0, seq_starts, kept)
-            ctx.scale = scale
-            ctx.state_dtype = None if initial_state is None else initial_state.dtype
+        out, state, kept = _forward(queries, keys, values, log_gates, betas, s0, scale, seq_starts, True)
+        ctx.save_for_backward(queries, keys, values, log_gates, betas, s0, seq_starts, kept)
+        ctx.scale = scale
+        ctx.state_dtype = None if initial_state is None else initial_state.dtype
         ctx.set_materialize_grads(False)
         return out, state
 
@@ -139,8 +140,12 @@ def scan(queries, keys, values, log_gates, betas, initial_state=None, scale=None
             raise RuntimeError(f"unsupported dtype {initial_state.dtype} of initial_state")
         if initial_state.device != queries.device:
             raise RuntimeError("all tensors must be on the same device")
-    return DeltaScan.apply(queries, keys, values, log_gates, betas, initial_state, K ** -0.5 if scale is None else float(scale),
-                           seq_starts)
+    scale = K ** -0.5 if scale is None else float(scale)
+    if torch.is_grad_enabled() and (queries.requires_grad or keys.requires_grad or values.requires_grad or log_gates.requires_grad
+                                    or betas.requires_grad or (initial_state is not None and initial_state.requires_grad)):
+        return DeltaScan.apply(queries, keys, values, log_gates, betas, initial_state, scale, seq_starts)
+    s0 = None if initial_state is None else initial_state.detach().float().contiguous()
+    return _forward(_dense_last(queries), _dense_last(keys), _dense_last(values), log_gates, betas, s0, scale, seq_starts, False)[:2]
 
 
 def step(queries, keys, values, log_gates, betas, state, slots=None, scale=None):
@@ -165,7 +170,8 @@ def step(queries, keys, values, log_gates, betas, state, slots=None, scale=None)
         raise RuntimeError("state must be float32")
     if state.device != queries.device:
         raise RuntimeError("all tensors must be on the same device")
-    if state.shape[0] and (not state[0].is_contiguous() or (state.shape[0] > 1 and state.stride(0) < H * K * V)):
+    if not state.is_contiguous() and state.shape[0] and (
+            not state[0].is_contiguous() or (state.shape[0] > 1 and state.stride(0) < H * K * V)):
         raise RuntimeError("the states of the pool must be contiguous")
     if slots is None:
         assert state.shape[0] >= B, "without slots the pool needs a state for each row"
@@ -176,7 +182,8 @@ def step(queries, keys, values, log_gates, betas, state, slots=None, scale=None)
         if slots.device != queries.device:
             raise RuntimeError("all tensors must be on the same device")
         slots = slots.contiguous()
-    if any(t.requires_grad for t in (queries, keys, values, log_gates, betas, state)) and torch.is_grad_enabled():
+    if torch.is_grad_enabled() and (queries.requires_grad or keys.requires_grad or values.requires_grad or log_gates.requires_grad
+                                    or betas.requires_grad or state.requires_grad):
         raise RuntimeError("step is not differentiable: call it under torch.no_grad()")
     out = torch.empty(B, H, V, dtype=values.dtype, device=values.device)
     if B:

@@ -30,22 +30,31 @@ def _rows(t, D):
     return r if r.stride(1) == 1 or D == 1 else r.contiguous()
 
 
+def _forward(rows, vectors, shape, activation, eps):
+    """rows: block_out, residual, gate; vectors: post_weight, scale, pre_weight."""
+    x = rows[0]
+    hidden = torch.empty(shape, dtype=x.dtype, device=x.device)
+    normed = None if vectors[2] is None else torch.empty(shape, dtype=x.dtype, device=x.device)
+    if x.shape[0]:
+        _native.norm_forward(_native.norm_args(*rows, *vectors, activation, eps), x.device, hidden, normed)
+    return (hidden, normed) if normed is not None else hidden
+
+
+def _dense(x, residual, gate, post_weight, scale, pre_weight):
+    D = x.shape[-1]
+    return ((_rows(x, D), _rows(residual, D), _rows(gate, D)),
+            tuple(w.contiguous() if isinstance(w, torch.Tensor) else w for w in (post_weight, scale, pre_weight)))
+
+
 class ResidualNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, residual, gate, post_weight, scale, pre_weight, activation, eps):
-        D = x.shape[-1]
-        rows = [_rows(t, D) for t in (x, residual, gate)]
-        vectors = [w.contiguous() if isinstance(w, torch.Tensor) else w for w in (post_weight, scale, pre_weight)]
-        hidden = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        normed = None if pre_weight is None else torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        if x.numel():
-            a = _native.norm_args(*rows, vectors[0], vectors[1], vectors[2], activation, eps)
-            _native.norm_forward(a, x.device, hidden, normed)
+        rows, vectors = _dense(x, residual, gate, post_weight, scale, pre_weight)
         ctx.save_for_backward(*rows, vectors[0], vectors[1] if isinstance(scale, torch.Tensor) else None, vectors[2])
         ctx.scale_value = None if isinstance(scale, torch.Tensor) else scale
         ctx.activation, ctx.eps, ctx.shape = activation, eps, x.shape
         ctx.set_materialize_grads(False)
-        return (hidden, normed) if normed is not None else hidden
+        return _forward(rows, vectors, x.shape, activation, eps)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
@@ -101,17 +110,18 @@ def residual_norm(block_out, residual=None, *, post_weight=None, gate=None, scal
         assert w.shape == (D,), "weights and a scale per channel must have shape (D,)"
         if w.dtype not in (x.dtype, torch.float32) or w.dtype != vectors[0].dtype:
             raise RuntimeError("weights and scale must all be of block_out's dtype or all float32")
-    for t in (x, residual, gate, *vectors):
-        if t is None:
-            continue
-        if not t.is_cuda:
-            raise RuntimeError("tensors must be CUDA tensors")
-        if t.device != x.device:
+    if not x.is_cuda:
+        raise RuntimeError("tensors must be CUDA tensors")
+    for t in (residual, gate, *vectors):
+        if t is not None and t.device != x.device:
             raise RuntimeError("all tensors must be on the same device")
     if not isinstance(scale, torch.Tensor):
         scale = 1.0 if scale is None else float(scale)
-    return ResidualNorm.apply(x, residual, gate, post_weight, scale, pre_weight,
-                              _ACTIVATIONS[activation], float(eps))
+    act, eps = _ACTIVATIONS[activation], float(eps)
+    if torch.is_grad_enabled() and any([isinstance(t, torch.Tensor) and t.requires_grad
+                                        for t in (x, residual, gate, post_weight, scale, pre_weight)]):
+        return ResidualNorm.apply(x, residual, gate, post_weight, scale, pre_weight, act, eps)
+    return _forward(*_dense(x, residual, gate, post_weight, scale, pre_weight), x.shape, act, eps)
 
 
 def gated_norm(x, gate, weight, activation="silu", eps=1e-6):

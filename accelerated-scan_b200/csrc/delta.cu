@@ -2,7 +2,7 @@
 // launches; and the kernel of single tokens.
 #include <atomic>
 
-#include "delta_common.cuh"
+#include "delta_tc.cuh"
 
 namespace ascan {
 
@@ -283,6 +283,186 @@ __global__ void __launch_bounds__(256) delta_step_kernel(StepParams p) {
     }
 }
 
+// The same for many rows: a head's K x V state is one dense block, so a persistent CTA takes it by one bulk copy into a
+// ring of shared-memory buffers, updates it there and sends it back by another, while the next ones arrive and the next
+// token's vectors are on their way to registers.  The kernel above asks for nothing while it reduces.  A warp takes 32
+// columns and every 4 N-th row, four rows at a time.
+constexpr int STEP_THREADS = 512, STEP_MAX_STAGES = 6, STEP_MAX_BATCH = 1024;
+
+struct StepRing {
+    int32_t stages, items;           // items: rows of the batch times heads
+    uint32_t bytes;                  // of a state
+    int *status;
+};
+
+__device__ __forceinline__ uint32_t load_raw(const void *p, int dtype, int64_t i) {
+    return dtype == ASCAN_F32 ? static_cast<const uint32_t *>(p)[i] : static_cast<const uint16_t *>(p)[i];
+}
+__device__ __forceinline__ float raw_value(uint32_t x, int dtype) {
+    if (dtype == ASCAN_F32) return __uint_as_float(x);
+    return dtype == ASCAN_BF16 ? __uint_as_float(x << 16) : __half2float(__ushort_as_half(static_cast<unsigned short>(x)));
+}
+
+__global__ void __launch_bounds__(STEP_THREADS, 1) delta_step_ring_kernel(const __grid_constant__ StepParams p, StepRing ring) {
+    extern __shared__ __align__(128) unsigned char dynamic[];
+    __shared__ float sk[128], sq[128], part_dot[4];
+    __shared__ __align__(16) float sums[2][16][32];      // [x, y][warp][column of its 32]
+    __shared__ uint64_t bars[STEP_MAX_STAGES];
+    __shared__ int slots[STEP_MAX_BATCH];                // -1: padded; -2: no such slot, or an earlier row has it
+    __shared__ int dead_flag;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int nv = p.V / 4, blocks = (nv + 7) / 8, block = warp % blocks, teams = 16 / blocks, team = warp / blocks;
+    const int cv = block * 8 + (lane & 7), row0 = team * 4 + (lane >> 3), rows = teams * 4;
+    const bool works = team < teams && cv < nv;
+    const uint32_t base = smem_addr(dynamic), bar0 = smem_addr(bars);
+    const Waiter wait = {&dead_flag, ring.status};
+    if (tid == 0) {
+        dead_flag = 0;
+        for (int i = 0; i < ring.stages; ++i) mbar_init(bar0 + 8 * i, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        fence_async_proxy();
+    }
+    for (int b = tid; b < p.batch; b += STEP_THREADS) {
+        const int64_t slot = read_slot(p, b);
+        slots[b] = slot < 0 ? -1 : slot >= p.pool ? -2 : static_cast<int>(slot);
+    }
+    __syncthreads();
+    int taken[STEP_MAX_BATCH / STEP_THREADS] = {};
+#pragma unroll
+    for (int j = 0; j < STEP_MAX_BATCH / STEP_THREADS; ++j) {
+        const int b = tid + j * STEP_THREADS;
+        if (p.slots && b < p.batch && slots[b] >= 0)
+            for (int i = 0; i < b; ++i) taken[j] |= slots[i] == slots[b];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < STEP_MAX_BATCH / STEP_THREADS; ++j)
+        if (taken[j]) slots[tid + j * STEP_THREADS] = -2;
+    __syncthreads();
+
+    const auto state_of = [&](int item) { return p.state + slots[item / p.H] * p.slot_stride + int64_t(item % p.H) * p.K * p.V; };
+    const auto ask = [&](int item, int stage) {          // one thread
+        const uint32_t bar = bar0 + 8 * stage;
+        if (slots[item / p.H] < 0) {
+            mbar_arrive(bar);
+            return;
+        }
+        mbar_expect(bar, ring.bytes);
+        asm volatile("cp.async.bulk.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                     :: "r"(base + stage * ring.bytes), "l"(state_of(item)), "r"(ring.bytes), "r"(bar) : "memory");
+    };
+    uint32_t rk = 0, rq = 0, rv[4] = {}, rg = 0, rb = 0;
+    const auto fetch = [&](int item) {                   // a token's vectors, as they are: a conversion would wait for them
+        const int b = item / p.H, h = item % p.H, hk = h / (p.H / p.Hk);
+        if (tid < p.K) {
+            rk = load_raw(p.k, p.dtype, b * p.k_s[0] + hk * p.k_s[1] + tid);
+            rq = load_raw(p.q, p.dtype, b * p.q_s[0] + hk * p.q_s[1] + tid);
+        }
+        rg = load_raw(p.g, p.g_dtype, b * p.g_s[0] + h * p.g_s[1]);
+        rb = load_raw(p.b, p.b_dtype, b * p.b_s[0] + h * p.b_s[1]);
+        if (works)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) rv[j] = load_raw(p.v, p.dtype, b * p.v_s[0] + h * p.v_s[1] + 4 * cv + j);
+    };
+    // one buffer less than there are is asked for ahead: the last one's way back ends while the next item is worked on
+    const int ahead = ring.stages - 1;
+    if (tid == 0)
+        for (int i = 0; i < ahead; ++i)
+            if (int(blockIdx.x) + i * int(gridDim.x) < ring.items) ask(blockIdx.x + i * gridDim.x, i);
+    if (int(blockIdx.x) < ring.items) fetch(blockIdx.x);
+    int stage = 0, turn = 0;
+    for (int item = blockIdx.x; item < ring.items; item += gridDim.x) {
+        const int b = item / p.H, h = item % p.H, slot = slots[b];
+        if (tid < 128) {
+            const float kv = tid < p.K ? raw_value(rk, p.dtype) : 0.f, qv = tid < p.K ? raw_value(rq, p.dtype) : 0.f;
+            sk[tid] = kv;
+            sq[tid] = qv;
+            float kq = kv * qv;
+#pragma unroll
+            for (int d = 16; d; d /= 2) kq += __shfl_xor_sync(~0u, kq, d);
+            if (lane == 0) part_dot[warp] = kq;
+        }
+        const float decay = expf(raw_value(rg, p.g_dtype)), beta = raw_value(rb, p.b_dtype);
+        float val[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) val[j] = raw_value(rv[j], p.dtype);
+        if (item + int64_t(gridDim.x) < ring.items) fetch(item + gridDim.x);
+        __syncthreads();
+        wait(bar0 + 8 * stage, turn & 1);
+        float4 *s = reinterpret_cast<float4 *>(dynamic + stage * ring.bytes) + cv;
+        float x[4] = {}, y[4] = {};
+        if (slot >= 0 && works) {
+#pragma unroll 4
+            for (int k = row0; k < p.K; k += rows) {
+                const float4 v = s[k * nv];
+                const float kv = sk[k], qv = sq[k];
+                x[0] += kv * v.x; x[1] += kv * v.y; x[2] += kv * v.z; x[3] += kv * v.w;
+                y[0] += qv * v.x; y[1] += qv * v.y; y[2] += qv * v.z; y[3] += qv * v.w;
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            x[j] += __shfl_xor_sync(~0u, x[j], 8);
+            y[j] += __shfl_xor_sync(~0u, y[j], 8);
+            x[j] += __shfl_xor_sync(~0u, x[j], 16);
+            y[j] += __shfl_xor_sync(~0u, y[j], 16);
+        }
+        if (lane < 8) {
+            *reinterpret_cast<float4 *>(&sums[0][warp][4 * lane]) = make_float4(x[0], x[1], x[2], x[3]);
+            *reinterpret_cast<float4 *>(&sums[1][warp][4 * lane]) = make_float4(y[0], y[1], y[2], y[3]);
+        }
+        __syncthreads();
+        if (slot >= 0 && works) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[j] = y[j] = 0.f;
+            for (int i = 0; i < teams; ++i) {
+                const float4 a = *reinterpret_cast<const float4 *>(&sums[0][i * blocks + block][4 * (lane & 7)]);
+                x[0] += a.x; x[1] += a.y; x[2] += a.z; x[3] += a.w;
+            }
+            float u[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) u[j] = beta * (val[j] - decay * x[j]);
+            if (row0 == 0) {
+                for (int i = 0; i < teams; ++i) {
+                    const float4 a = *reinterpret_cast<const float4 *>(&sums[1][i * blocks + block][4 * (lane & 7)]);
+                    y[0] += a.x; y[1] += a.y; y[2] += a.z; y[3] += a.w;
+                }
+                const float dot = (part_dot[0] + part_dot[1]) + (part_dot[2] + part_dot[3]);
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    store_from_float(p.out, p.dtype, (int64_t(b) * p.H + h) * p.V + 4 * cv + j, p.scale * (decay * y[j] + dot * u[j]));
+            }
+#pragma unroll 4
+            for (int k = row0; k < p.K; k += rows) {
+                float4 v = s[k * nv];
+                const float kv = sk[k];
+                v.x = decay * v.x + kv * u[0]; v.y = decay * v.y + kv * u[1]; v.z = decay * v.z + kv * u[2]; v.w = decay * v.w + kv * u[3];
+                s[k * nv] = v;
+            }
+            fence_async_proxy();
+        } else if (slot < 0 && works && row0 == 0) {         // as in the kernel above
+            const float o = slot == -1 ? 0.f : __int_as_float(0x7fc00000);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) store_from_float(p.out, p.dtype, (int64_t(b) * p.H + h) * p.V + 4 * cv + j, o);
+        }
+        __syncthreads();
+        if (tid == 0) {
+            if (slot >= 0)
+                asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;"
+                             :: "l"(state_of(item)), "r"(base + stage * ring.bytes), "r"(ring.bytes) : "memory");
+            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+            asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");      // the item before this one has left its buffer
+            const int64_t next = int64_t(item) + int64_t(ahead) * gridDim.x;
+            if (next < ring.items) ask(static_cast<int>(next), stage == 0 ? ring.stages - 1 : stage - 1);
+        }
+        if (++stage == ring.stages) {
+            stage = 0;
+            ++turn;
+        }
+    }
+    if (tid == 0) tma_store_done();
+}
+
 }  // namespace ascan
 
 using namespace ascan;
@@ -387,7 +567,7 @@ int ascan_delta_step(const ascan_delta_token *a, void *out, float *state, int64_
     if (!slots && pool < a->batch) return ASCAN_ERR_INVALID_ARG;
     const int64_t inner = int64_t(a->heads) * a->k_dim * a->v_dim;
     if (slot_stride < inner) return ASCAN_ERR_INVALID_ARG;
-    const int64_t grid = a->batch * a->heads * ((a->v_dim + 31) / 32);
+    const int64_t grid = a->batch * a->heads * ((int64_t(a->v_dim) + 31) / 32);
     if (grid > 0x7fffffff || a->batch > 0x7fffffff) return ASCAN_ERR_UNSUPPORTED;
     StepParams p = {};
     p.q = a->queries; p.k = a->keys; p.v = a->values; p.g = a->log_gates; p.b = a->betas;
@@ -409,8 +589,22 @@ int ascan_delta_step(const ascan_delta_token *a, void *out, float *state, int64_
     p.scale = a->scale;
     p.out = out;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    // 16-byte accesses need rows of the state that start on 16 bytes
-    if (p.V % 4 == 0 && slot_stride % 4 == 0 && (reinterpret_cast<uintptr_t>(state) & 15) == 0)
+    // 16-byte accesses need rows of the state that start on 16 bytes; the ring needs states of which three fit into shared
+    // memory, and pays from about two states an SM on (fewer are spread over more CTAs, each with a piece)
+    const bool aligned = p.V % 4 == 0 && slot_stride % 4 == 0 && (reinterpret_cast<uintptr_t>(state) & 15) == 0;
+    int sms = 0;
+    const int rc = delta_sm_count(&sms);
+    if (rc != ASCAN_OK) return rc;
+    const int64_t items = a->batch * a->heads, bytes = int64_t(p.K) * p.V * 4;
+    if (aligned && p.V <= 512 && bytes <= 65536 && a->batch <= STEP_MAX_BATCH && pool <= 0x7fffffff && items >= 2 * sms) {
+        int stages = static_cast<int>(200 * 1024 / bytes);
+        if (stages > STEP_MAX_STAGES) stages = STEP_MAX_STAGES;
+        const StepRing ring = {stages, static_cast<int32_t>(items), static_cast<uint32_t>(bytes), a->status};
+        const int smem = static_cast<int>(stages * bytes);
+        if (cudaFuncSetAttribute(delta_step_ring_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024) != cudaSuccess)
+            return ASCAN_ERR_LAUNCH;
+        delta_step_ring_kernel<<<sms, STEP_THREADS, smem, st>>>(p, ring);
+    } else if (p.V % 4 == 0 && slot_stride % 4 == 0 && (reinterpret_cast<uintptr_t>(state) & 15) == 0)
         delta_step_kernel<4><<<unsigned(grid), 256, 0, st>>>(p);
     else
         delta_step_kernel<1><<<unsigned(grid), 256, 0, st>>>(p);

@@ -1,10 +1,11 @@
 // Gated delta rule, forward sweep on tcgen05: bf16 inputs, one CTA a sequence, head and 128 columns of V.
 //
 // The state is held transposed: rows of tensor memory and threads are columns of V, so that all products of a chunk
-//     x = V^T - gam (S^T K^T);   e = x - (beta x) M^T;   dS^T = (Gam_C u) K;   out = scale gam (S^T Q^T) + u P^T
+//     x = V^T - gam (S^T K^T);   e = x - x (M beta)^T;   dS^T = (Gam_C u) K;   out = scale gam (S^T Q^T) + u P^T
 // have 128 rows, and their left operands come from tensor memory, where the threads that computed them (256: two for each
 // row, half of the columns each) put them as bf16 terms.  The fp32 state itself stays in those threads' registers.  Terms
-// are chosen as in the warp-level sweep: two for whatever reaches the state, one for what reaches out alone.
+// are chosen as in the warp-level sweep: two for whatever reaches the state; for out alone S and P are one, u is two (of the
+// three, S matters least: out was 2.9e-3 off with one term each, 2.4e-3 so, 1.7e-3 of it its own rounding).
 //
 // Two more groups of four warps prepare M and P, each of every other chunk, up to two chunks ahead; one warp loads the
 // tiles (three stages), one runs the gates' sums and one issues.  Products that the
@@ -88,7 +89,7 @@ struct TcForward {
     // columns of tensor memory
     static constexpr int S = 0, X = 128, BX = 192, D2 = 256, O1 = 320, O2 = 384, KK = 448;
 };
-enum : int { B_TILE = 0, B_PREP = 3, B_GATES = 5, B_KK = 8, B_MP = 10, B_X = 12, B_D2, B_S, B_O, B_AS, B_BX, B_U, B_OREAD, B_KREAD, B_FREE, B_TAIL = B_FREE + 3, B_COUNT };
+enum : int { B_TILE = 0, B_PREP = 3, B_GATES = 5, B_KK = 8, B_MP = 10, B_X = 12, B_D2, B_S, B_O, B_AS, B_BX, B_U, B_UO, B_OREAD, B_KREAD, B_FREE, B_TAIL = B_FREE + 3, B_COUNT };
 
 constexpr int TC_THREADS = 20 * 32;
 // Registers a thread: 96 at launch; 152 * 256 + 64 * 256 + 48 * 128 = 96 * 640
@@ -188,11 +189,11 @@ __global__ void __launch_bounds__(TC_THREADS, 1) delta_sweep_tc_kernel(const __g
 #pragma unroll
                 for (int j = 0; j < 8; j += 2) {
                     const int i = 8 * q + j;
-                    const ulonglong2 ga = scalars(SC_GAM, 2 * i), be = scalars(SC_BETA, 2 * i);
+                    const ulonglong2 ga = scalars(SC_GAM, 2 * i);
                     x[i] = fma2(ga.x, two_bits(r[2 * i], r[2 * i + 1]), x[i]);
                     x[i + 1] = fma2(ga.y, two_bits(r[2 * i + 2], r[2 * i + 3]), x[i + 1]);
-                    split_f2(mul2(be.x, x[i]), hi[j], lo[j]);
-                    split_f2(mul2(be.y, x[i + 1]), hi[j + 1], lo[j + 1]);
+                    split_f2(x[i], hi[j], lo[j]);
+                    split_f2(x[i + 1], hi[j + 1], lo[j + 1]);
                 }
                 tmem_st8(t0 + L::BX + 16 * part + 8 * q, hi);
                 tmem_st8(t0 + L::BX + 32 + 16 * part + 8 * q, lo);
@@ -204,24 +205,34 @@ __global__ void __launch_bounds__(TC_THREADS, 1) delta_sweep_tc_kernel(const __g
             tc_wait_ld();
 #pragma unroll
             for (int q = 0; q < 2; ++q) {
-                uint32_t u[8], hi[8], lo[8];
+                uint32_t hi[8], lo[8];
 #pragma unroll
                 for (int j = 0; j < 8; j += 2) {
                     const int i = 8 * q + j;
-                    const ulonglong2 gc = scalars(SC_GAMC, 2 * i), be = scalars(SC_BETA, 2 * i);
+                    const ulonglong2 gb = scalars(SC_GAMC_BETA, 2 * i);
                     x[i] = add2(x[i], two_bits(r[2 * i], r[2 * i + 1]));
                     x[i + 1] = add2(x[i + 1], two_bits(r[2 * i + 2], r[2 * i + 3]));
-                    const f2 u0 = mul2(be.x, x[i]), u1 = mul2(be.y, x[i + 1]);
-                    u[j] = pack_f2(u0);
-                    u[j + 1] = pack_f2(u1);
-                    split_f2(mul2(gc.x, u0), hi[j], lo[j]);
-                    split_f2(mul2(gc.y, u1), hi[j + 1], lo[j + 1]);
+                    split_f2(mul2(gb.x, x[i]), hi[j], lo[j]);
+                    split_f2(mul2(gb.y, x[i + 1]), hi[j + 1], lo[j + 1]);
                 }
                 tmem_st8(t0 + L::X + 16 * part + 8 * q, hi);
                 tmem_st8(t0 + L::X + 32 + 16 * part + 8 * q, lo);
-                tmem_st8(t0 + L::BX + 16 * part + 8 * q, u);
             }
             hand_over(B_U);
+            // u for out, while the state's product runs
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                uint32_t hi[8], lo[8];
+#pragma unroll
+                for (int j = 0; j < 8; j += 2) {
+                    const ulonglong2 be = scalars(SC_BETA, 16 * q + 2 * j);
+                    split_f2(mul2(be.x, x[8 * q + j]), hi[j], lo[j]);
+                    split_f2(mul2(be.y, x[8 * q + j + 1]), hi[j + 1], lo[j + 1]);
+                }
+                tmem_st8(t0 + L::BX + 16 * part + 8 * q, hi);
+                tmem_st8(t0 + L::BX + 32 + 16 * part + 8 * q, lo);
+            }
+            hand_over(B_UO);
             const int64_t at = int64_t(sq.slot0 + c) * p.H + h;
             if (SAVE && v0 + v < p.Vp) {
                 uint4 *o = reinterpret_cast<uint4 *>(p.e + (at * p.Vp + v0 + v) * 64 + 32 * part);
@@ -317,7 +328,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) delta_sweep_tc_kernel(const __g
             if (c >= 2) wait(bar(B_MP + team), ((c - 2) >> 1) & 1);
             wait(bar(B_KK + team), (c >> 1) & 1);
             tc_fence_after();
-            decayed_row(row, f, factor, l_row ? i : i + 1, gs, i, t, [&](int bj, const float (&x)[16]) {
+            decayed_row(row, f, factor, l_row, !l_row, gs, i, t, [&](int bj, const float (&x)[16]) {
                 if (l_row) {
 #pragma unroll
                     for (int j = 0; j < 16; j += 4)
@@ -334,7 +345,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) delta_sweep_tc_kernel(const __g
             __syncwarp();
             if (lane == 0) mbar_arrive(bar(B_KREAD));
             sync();
-            make_m(m, gs.sc + SC_BETA * 64, t, sync);
+            make_m(m, t, sync);
             fence_async_proxy();
             mbar_arrive(bar(B_PREP + team));
         }
@@ -420,7 +431,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) delta_sweep_tc_kernel(const __g
                 wait(bar(B_PREP + (c & 1)), (c >> 1) & 1);
                 wait(bar(B_BX), c & 1);
                 tc_fence_after();
-                // tokens 16 t .. of beta x reach the tokens from 16 t on only
+                // tokens 16 t .. of x reach the tokens from 16 t on only
 #pragma unroll
                 for (int t = 0; t < 4; ++t) {
                     const uint32_t desc = mma_desc(64 - 16 * t, false, true), d = tmem + L::D2 + 16 * t, at = (16 * t * 128 + 32 * t) >> 4;
@@ -437,10 +448,14 @@ __global__ void __launch_bounds__(TC_THREADS, 1) delta_sweep_tc_kernel(const __g
                     for (int lo = 0; lo < 2; ++lo)
                         tc_mma_ts(tmem + L::S, tmem + L::X + 32 * lo + 8 * t, down + kq(0, 16 * t), mma_desc(KP, true), t + lo > 0);
                 tc_commit(bar(B_S));
+                wait(bar(B_UO), c & 1);
+                tc_fence_after();
 #pragma unroll
                 for (int t = 0; t < 4; ++t)
-                    tc_mma_ts(tmem + L::O2 + 16 * t, tmem + L::BX + 8 * t, m + ((L::P + 16 * t * 128 + 32 * t) >> 4),
-                              mma_desc(64 - 16 * t, false), t > 0);
+#pragma unroll
+                    for (int lo = 0; lo < 2; ++lo)
+                        tc_mma_ts(tmem + L::O2 + 16 * t, tmem + L::BX + 32 * lo + 8 * t, m + ((L::P + 16 * t * 128 + 32 * t) >> 4),
+                                  mma_desc(64 - 16 * t, false), t + lo > 0);
                 tc_commit(bar(B_O));
                 tc_commit(bar(B_MP + (c & 1)));
                 tc_commit(bar(B_FREE + stage));

@@ -183,23 +183,26 @@ __device__ __forceinline__ void tma_store_done() { asm volatile("cp.async.bulk.w
 // ---- preparing a chunk -----------------------------------------------------------------------------------------------
 //
 // 128 threads.  K K^T and Q K^T of the chunk come from one product of 128 rows ([K; Q]) in tensor memory, a row a
-// thread.  M = L (I + diag(beta) L)^{-1} by halves: for the lower left block between two finished ones,
-//     M21 = (I - M22 beta2) L21 (I - beta1 M11),
-// from 16 x 16 blocks (substitution, a column a thread) to 32 and 64 on warp matrix instructions with two-term operands
-// (2^-16, as M itself is handed on).
+// thread.  Here L carries the factor beta on its columns (forward) or rows (backward), and with it M: N = M diag(beta) =
+// L' (I + L')^{-1} for L' = L diag(beta), or diag(beta) M likewise.  By halves: for the lower left block between two
+// finished ones,
+//     N21 = (I - N22) L'21 (I - N11),
+// from 4 x 4 (substitution) to 8 and 16 in fp32, to 32 and 64 on warp matrix instructions with two-term operands
+// (2^-16, as N itself is handed on).
 
 constexpr int PITCH = 68;                        // floats a row of M
 constexpr int M_BYTES = 64 * PITCH * 4;          // 17 KB: also the place of M's two tiles
-enum : int { SC_OUT = SC_ARRAYS, SC_SHARED = SC_ARRAYS + 1 };     // in shared memory also scale * gam
+enum : int { SC_OUT = SC_ARRAYS, SC_GAMC_BETA, SC_SHARED };      // in shared memory also scale * gam and Gam_C * beta
 struct GateShared {                              // of one chunk
     float sc[SC_SHARED * 64];
-    float w[2][64];                              // for token j in a block of 16: e^{G_end - G_j}, and e^{G_first - G_j}
+    float w[2][2][64];                           // for token j in a block of 16: e^{G_end - G_j}, and e^{G_first - G_j};
+                                                 // [1]: times beta_j
     int direct[4];                               // blocks whose decay leaves the range of the second
 };
 
-// 16 x 16 blocks of fp32 in shared memory (PITCH floats a row): to = from - (A diag(beta)) B over `steps` blocks of A's
-// columns and B's rows.  One warp.
-__device__ __forceinline__ void block_product(float *to, const float *from, const float *A, const float *beta, const float *B, int steps) {
+// 16 x 16 blocks of fp32 in shared memory (PITCH floats a row): to = from - A B over `steps` blocks of A's columns and B's
+// rows.  One warp.
+__device__ __forceinline__ void block_product(float *to, const float *from, const float *A, const float *B, int steps) {
     const int lane = threadIdx.x & 31, g = lane >> 2, t2 = 2 * (lane & 3);
     float c[2][2][4];                            // two sums a tile, so that products need not wait for one another
 #pragma unroll
@@ -212,13 +215,13 @@ __device__ __forceinline__ void block_product(float *to, const float *from, cons
             c[1][n][2 * h] = c[1][n][2 * h + 1] = 0.f;
         }
 #pragma unroll 1
-    for (int k = 0; k < steps; ++k, A += 16, beta += 16, B += 16 * PITCH) {
+    for (int k = 0; k < steps; ++k, A += 16, B += 16 * PITCH) {
         uint32_t a[2][4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const int col = (j >> 1) * 8 + t2;
             const float2 x = *reinterpret_cast<const float2 *>(A + (g + (j & 1) * 8) * PITCH + col);
-            split2(-x.x * beta[col], -x.y * beta[col + 1], a[0][j], a[1][j]);
+            split2(-x.x, -x.y, a[0][j], a[1][j]);
         }
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
@@ -272,13 +275,18 @@ __device__ __forceinline__ void chunk_gates(const float (&g)[2], const float (&b
         const float hi = float(G), gam = R == 0 ? expf(hi) : 0.f, back = float(first - G);
         sc[SC_GAM * 64 + i] = gam;
         sc[SC_OUT * 64 + i] = scale * gam;
-        sc[SC_GAMC * 64 + i] = R == all ? expf(float(last - G)) : 0.f;
+        const float gam_c = R == all ? expf(float(last - G)) : 0.f;
+        sc[SC_GAMC * 64 + i] = gam_c;
+        sc[SC_GAMC_BETA * 64 + i] = gam_c * beta[j];
         sc[SC_BETA * 64 + i] = beta[j];
         sc[SC_GHI * 64 + i] = hi;
         sc[SC_GLO * 64 + i] = float(G - double(hi));
         sc[SC_RESET * 64 + i] = float(R);
-        gs.w[0][i] = R == r_end ? expf(float(end - G)) : 0.f;
-        gs.w[1][i] = expf(back);
+        const float to_end = R == r_end ? expf(float(end - G)) : 0.f, to_first = expf(back);
+        gs.w[0][0][i] = to_end;
+        gs.w[0][1][i] = to_first;
+        gs.w[1][0][i] = to_end * beta[j];
+        gs.w[1][1][i] = to_first * beta[j];
         plain = plain && fabsf(back) <= 60.f;
     }
     const unsigned ok = __ballot_sync(~0u, plain);
@@ -298,18 +306,18 @@ __device__ __forceinline__ void row_factors(float (&f)[4][128], float factor, co
                                                             sc[SC_GHI * 64 + ref], sc[SC_GLO * 64 + ref], sc[SC_RESET * 64 + ref]);
     }
 }
-// put(bj, x) gets 16 values of block bj.  A warp has the rows of two blocks and skips what lies above both.  Tokens from
-// `stop` on get zero.
+// put(bj, x) gets 16 values of block bj, times beta of their tokens where `columns`.  A warp has the rows of two blocks and
+// skips what lies above both.  Where `mask`, values above the diagonal (which stays) are zero; else they are anything.
 template <class PUT>
-__device__ __forceinline__ void decayed_row(uint32_t tmem, const float (&f)[4][128], float factor, int stop, const GateShared &gs, int i,
-                                            int tid, PUT put) {
+__device__ __forceinline__ void decayed_row(uint32_t tmem, const float (&f)[4][128], float factor, bool columns, bool mask,
+                                            const GateShared &gs, int i, int tid, PUT put) {
     const float *sc = gs.sc;
     const int bi = i >> 4, b1 = i >> 5 << 1 | 1;         // b1: the warp's last own block
 #pragma unroll 1
     for (int bj = 0; bj <= b1; ++bj) {
         uint32_t r[16];
         tmem_ld16(r, tmem + 16 * bj);
-        const float *w = gs.w[bj == bi] + 16 * bj;
+        const float *w = gs.w[columns][bj == bi] + 16 * bj;
         const f2 ff = two(f[bj][tid], f[bj][tid]);
         float x[16];
         tc_wait_ld();
@@ -324,38 +332,39 @@ __device__ __forceinline__ void decayed_row(uint32_t tmem, const float (&f)[4][1
 #pragma unroll 1
             for (int j = 0; j < 16; ++j) {
                 const int t = 16 * bj + j;
-                const float d = factor * decay_between(sc[SC_GHI * 64 + i], sc[SC_GLO * 64 + i], sc[SC_RESET * 64 + i], sc[SC_GHI * 64 + t],
-                                                       sc[SC_GLO * 64 + t], sc[SC_RESET * 64 + t]);
+                const float d = factor * (columns ? sc[SC_BETA * 64 + t] : 1.f) *
+                    decay_between(sc[SC_GHI * 64 + i], sc[SC_GLO * 64 + i], sc[SC_RESET * 64 + i], sc[SC_GHI * 64 + t], sc[SC_GLO * 64 + t],
+                                  sc[SC_RESET * 64 + t]);
 #pragma unroll
                 for (int k = 0; k < 16; ++k)
                     if (k == j) x[k] = d * __uint_as_float(r[k]);
             }
         }
-        if (bj >= b1 - 1)
+        if (mask && bj >= b1 - 1)
 #pragma unroll
-            for (int j = 0; j < 16; ++j) x[j] = 16 * bj + j < stop ? x[j] : 0.f;
+            for (int j = 0; j < 16; ++j) x[j] = 16 * bj + j <= i ? x[j] : 0.f;
         put(bj, x);
     }
 }
 
-// From L (shared, fp32, 64 rows of PITCH) to M as two bf16 tiles, hi and lo, in its place; all 128 threads, SYNC a barrier of
-// theirs.  On entry the diagonal blocks of 16 are zero above the diagonal; the upper right quarter is scratch.
+// From L (shared, fp32, 64 rows of PITCH) to N = L (I + L)^{-1} as two bf16 tiles, hi and lo, in its place; all 128 threads,
+// SYNC a barrier of theirs.  What lies above L's diagonal is not read; the upper right quarter is scratch.
 template <class SYNC>
-__device__ __forceinline__ void make_m(float *m, const float *beta, int tid, SYNC sync) {
+__device__ __forceinline__ void make_m(float *m, int tid, SYNC sync) {
     const int lane = tid & 31, warp = tid >> 5;
     const auto block = [&](int r, int col) { return m + 16 * r * PITCH + 16 * col; };
     {   // a diagonal block a warp: 4 x 4 blocks by substitution, then two steps of the same kind as below
         float *d = block(warp, warp), *t = block(warp >> 1, 2 + (warp & 1));
-        const float *be = beta + 16 * warp;
         if (lane < 16) {
             const int c = lane & 3;
             float *x = d + (lane >> 2) * 4 * (PITCH + 1);
-            const float *b4 = be + (lane >> 2) * 4;
             const float l21 = x[2 * PITCH + 1], l31 = x[3 * PITCH + 1], l32 = x[3 * PITCH + 2];
-            const float m1 = c < 1 ? x[PITCH + c] : 0.f, t1 = b4[1] * m1;
-            const float m2 = (c < 2 ? x[2 * PITCH + c] : 0.f) - l21 * t1;
-            const float m3 = (c < 3 ? x[3 * PITCH + c] : 0.f) - l31 * t1 - l32 * (b4[2] * m2);
+            const float m1 = c < 1 ? x[PITCH + c] : 0.f;
+            const float m2 = (c < 2 ? x[2 * PITCH + c] : 0.f) - l21 * m1;
+            const float m3 = (c < 3 ? x[3 * PITCH + c] : 0.f) - l31 * m1 - l32 * m2;
             __syncwarp(0xffff);
+            x[c] = 0.f;
+            x[PITCH + c] = m1;
             x[2 * PITCH + c] = m2;
             x[3 * PITCH + c] = m3;
         }
@@ -364,36 +373,41 @@ __device__ __forceinline__ void make_m(float *m, const float *beta, int tid, SYN
             const int r = lane >> 2 & 3, c = lane & 3, o = (lane >> 4) * 8;
             float *low = d + (o + 4) * PITCH + o;
             float y = low[r * PITCH + c];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) y -= low[r * PITCH + k] * be[o + k] * d[(o + k) * PITCH + o + c];
+            const float4 a = *reinterpret_cast<const float4 *>(low + r * PITCH);
+            const float *x = d + o * PITCH + o + c;
+            y -= a.x * x[0] + a.y * x[PITCH] + a.z * x[2 * PITCH] + a.w * x[3 * PITCH];
             t[(o + r) * PITCH + c] = y;
             __syncwarp();
-#pragma unroll
-            for (int k = 0; k < 4; ++k) y -= low[r * PITCH + 4 + k] * be[o + 4 + k] * t[(o + k) * PITCH + c];
+            const float4 b = *reinterpret_cast<const float4 *>(low + r * PITCH + 4);
+            const float *z = t + o * PITCH + c;
+            y -= b.x * z[0] + b.y * z[PITCH] + b.z * z[2 * PITCH] + b.w * z[3 * PITCH];
             low[r * PITCH + c] = y;
+            d[(o + r) * PITCH + o + 4 + c] = 0.f;
         }
         __syncwarp();
         {
             const int r = lane >> 2, c = 2 * (lane & 3);
             float *low = d + 8 * PITCH;
             float2 y = *reinterpret_cast<const float2 *>(low + r * PITCH + c);
+            const auto subtract = [&](const float *row, const float *x) {
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                const float a = low[r * PITCH + k] * be[k];
-                const float2 x = *reinterpret_cast<const float2 *>(d + k * PITCH + c);
-                y.x -= a * x.x;
-                y.y -= a * x.y;
-            }
+                for (int k = 0; k < 8; k += 4) {
+                    const float4 a = *reinterpret_cast<const float4 *>(row + k);
+                    const float a4[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const float2 v = *reinterpret_cast<const float2 *>(x + (k + j) * PITCH + c);
+                        y.x -= a4[j] * v.x;
+                        y.y -= a4[j] * v.y;
+                    }
+                }
+            };
+            subtract(low + r * PITCH, d);
             *reinterpret_cast<float2 *>(t + r * PITCH + c) = y;
             __syncwarp();
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                const float a = low[r * PITCH + 8 + k] * be[8 + k];
-                const float2 x = *reinterpret_cast<const float2 *>(t + k * PITCH + c);
-                y.x -= a * x.x;
-                y.y -= a * x.y;
-            }
+            subtract(low + r * PITCH + 8, t);
             *reinterpret_cast<float2 *>(low + r * PITCH + c) = y;
+            *reinterpret_cast<float2 *>(d + r * PITCH + 8 + c) = make_float2(0.f, 0.f);
         }
     }
     sync();
@@ -409,7 +423,6 @@ __device__ __forceinline__ void make_m(float *m, const float *beta, int tid, SYN
         if (step >= 2 || warp < 2)
             block_product(first ? block(up, right) : block(low, left), first ? block(low, left) : block(up, right),
                           first ? block(low, left) : step < 2 ? block(low, low) : block(low, 2),
-                          beta + 16 * (first ? left : step < 2 ? low : 2),
                           first ? block(left, left) : step < 2 ? block(up, right) : block(0, right),
                           step < 2 ? 1 : first ? 2 - q : 1 + r);
         sync();
@@ -427,7 +440,7 @@ __device__ __forceinline__ void make_m(float *m, const float *beta, int tid, SYN
         uint32_t h[4], l[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-            split2(col + 2 * j < row ? x[2 * j] : 0.f, col + 2 * j + 1 < row ? x[2 * j + 1] : 0.f, h[j], l[j]);
+            split2(x[2 * j], x[2 * j + 1], h[j], l[j]);
         *reinterpret_cast<uint4 *>(tiles + tile_off<8>(row, col >> 3)) = make_uint4(h[0], h[1], h[2], h[3]);
         *reinterpret_cast<uint4 *>(tiles + 8192 + tile_off<8>(row, col >> 3)) = make_uint4(l[0], l[1], l[2], l[3]);
     }

@@ -5,12 +5,12 @@
 // and its gradients.  Everything is bound by memory: the forward reads x, residual and gate and writes h and y, the
 // backward reads x, residual, gate and the two gradients and writes three; a row stays in registers between its
 // reductions.  The backward recomputes h from the inputs (the same bytes as reading a saved one), so that no sum sees a
-// rounded h.  A thread holds eight neighbouring elements, 16 bytes at a time;
+// rounded h.  A thread holds eight elements (sixteen in the forward of long rows), 16 bytes at a time;
 // G threads share a row, and a CTA keeps the weights, and in the backward the weights' gradients, in registers over all
 // its rows.  Sums of the weights' gradients over CTAs are a second launch, in a fixed order.
 #include <atomic>
 
-#include "delta_common.cuh"
+#include "delta_tc.cuh"
 
 namespace ascan {
 
@@ -23,10 +23,11 @@ struct NormParams {
     const void *d_hidden, *d_normed;
     void *d_x, *d_residual, *d_gate;
     float *partial;                                 // [grid][3][D]: post, scale, pre
+    int32_t stages;                                 // of the copies' ring; 0: plain loads
+    int *status;                                    // nullable: set when a wait for a copy expired
 };
 
-constexpr int EPT = 8;                              // elements a thread holds
-constexpr int NORM_THREADS = 1024, NORM_MAX_D = EPT * NORM_THREADS;
+constexpr int NORM_THREADS = 1024, NORM_MAX_D = 8 * NORM_THREADS;
 constexpr int NORM_NARROW = 512;                    // threads up to which the backward keeps all it needs in registers
 
 enum : int { ACT_NONE = 0, ACT_SIGMOID = 1, ACT_SILU = 2 };
@@ -79,104 +80,242 @@ template <> struct Elem<__half> {
     static __device__ __half put(float v) { return __float2half_rn(v); }
 };
 
-// Where a thread's elements lie in a row: EPT neighbours (ALIGNED), or every G-th element.
-template <bool ALIGNED>
-__device__ __forceinline__ int element(int i, int gt, int G) { return ALIGNED ? gt * EPT + i : gt + i * G; }
-
+// Where a thread's E elements lie in a row: pieces of 16 bytes, G pieces apart, or every G-th element (not ALIGNED).
 template <class T, bool ALIGNED>
-__device__ __forceinline__ void load_row(const void *src, int64_t at, int gt, int G, int D, float (&x)[EPT]) {
+__device__ __forceinline__ int element(int i, int gt, int G) {
+    constexpr int VEC = Elem<T>::VEC;
+    return ALIGNED ? (i / VEC * G + gt) * VEC + i % VEC : gt + i * G;
+}
+
+template <class T, bool ALIGNED, int E>
+__device__ __forceinline__ void load_row(const void *src, int64_t at, int gt, int G, int D, float (&x)[E]) {
     const T *s = static_cast<const T *>(src) + at;
     if (ALIGNED) {
         constexpr int VEC = Elem<T>::VEC;
 #pragma unroll
-        for (int i = 0; i < EPT; i += VEC) {
+        for (int i = 0; i < E; i += VEC) {
             uint4 r = make_uint4(0, 0, 0, 0);
-            if (gt * EPT + i < D) r = __ldcs(reinterpret_cast<const uint4 *>(s + gt * EPT + i));
+            const int e = element<T, true>(i, gt, G);
+            if (e < D) r = __ldcs(reinterpret_cast<const uint4 *>(s + e));
             Elem<T>::unpack(r, x + i);
         }
     } else {
 #pragma unroll
-        for (int i = 0; i < EPT; ++i) x[i] = gt + i * G < D ? Elem<T>::get(s[gt + i * G]) : 0.f;
+        for (int i = 0; i < E; ++i) x[i] = gt + i * G < D ? Elem<T>::get(s[gt + i * G]) : 0.f;
     }
 }
 
-template <class T, bool ALIGNED>
-__device__ __forceinline__ void store_row(void *dst, int64_t at, int gt, int G, int D, const float (&x)[EPT]) {
+template <class T, bool ALIGNED, int E>
+__device__ __forceinline__ void store_row(void *dst, int64_t at, int gt, int G, int D, const float (&x)[E]) {
     T *s = static_cast<T *>(dst) + at;
     if (ALIGNED) {
         constexpr int VEC = Elem<T>::VEC;
 #pragma unroll
-        for (int i = 0; i < EPT; i += VEC)
-            if (gt * EPT + i < D) *reinterpret_cast<uint4 *>(s + gt * EPT + i) = Elem<T>::pack(x + i);
+        for (int i = 0; i < E; i += VEC) {
+            const int e = element<T, true>(i, gt, G);
+            if (e < D) *reinterpret_cast<uint4 *>(s + e) = Elem<T>::pack(x + i);
+        }
     } else {
 #pragma unroll
-        for (int i = 0; i < EPT; ++i)
+        for (int i = 0; i < E; ++i)
             if (gt + i * G < D) s[gt + i * G] = Elem<T>::put(x[i]);
     }
 }
 
-template <bool ALIGNED>
-__device__ __forceinline__ void load_weight(const void *w, int dtype, int gt, int G, int D, float missing, float (&x)[EPT]) {
+// Rows by bulk copies: a ring of `stages` buffers, each the rows that the CTA works on at once (`slots`) of every input, so
+// that the next rows are under way while these are reduced: with plain loads a CTA asks for nothing between its first
+// barrier and its last store.  One thread issues; rows that lie dense are one copy an input.
+template <class T, int INPUTS>
+struct RowRing {
+    const NormParams &p;
+    const void *src[INPUTS];
+    int64_t stride[INPUTS];
+    int slots, stage = 0, turn = 0;
+    uint32_t base, bars, bytes;          // bytes: of an input in a buffer
+    unsigned char *mem;
+    volatile int *dead;
+    int64_t next;                        // first row that has not been asked for
+
+    __device__ __forceinline__ RowRing(const NormParams &params, unsigned char *smem, uint64_t *bar, int *gave_up, int slots_)
+        : p(params), slots(slots_), bars(smem_addr(bar)), mem(smem), dead(gave_up) {
+        base = smem_addr(smem);
+        bytes = uint32_t(slots) * p.D * sizeof(T);
+        next = int64_t(blockIdx.x) * slots;
+    }
+    __device__ __forceinline__ void init() {
+        if (threadIdx.x == 0) {
+            *dead = 0;
+            for (int i = 0; i < p.stages; ++i) mbar_init(bars + 8 * i, 1);
+            asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+            fence_async_proxy();
+        }
+        __syncthreads();
+        if (threadIdx.x == 0)
+            for (int i = 0; i < p.stages; ++i) issue(i);
+    }
+    __device__ __forceinline__ void copy(uint32_t dst, const void *from, uint32_t n, uint32_t bar) {
+        asm volatile("cp.async.bulk.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                     :: "r"(dst), "l"(from), "r"(n), "r"(bar) : "memory");
+    }
+    __device__ __forceinline__ void issue(int s) {       // one thread
+        if (next >= p.rows) return;
+        const int rows = static_cast<int>(p.rows - next < slots ? p.rows - next : slots);
+        uint32_t total = 0;
 #pragma unroll
-    for (int i = 0; i < EPT; ++i) {
-        const int e = element<ALIGNED>(i, gt, G);
+        for (int i = 0; i < INPUTS; ++i) total += src[i] ? rows * p.D * uint32_t(sizeof(T)) : 0;
+        mbar_expect(bars + 8 * s, total);
+#pragma unroll
+        for (int i = 0; i < INPUTS; ++i) {
+            if (!src[i]) continue;
+            const T *from = static_cast<const T *>(src[i]) + next * stride[i];
+            const uint32_t dst = base + (s * INPUTS + i) * bytes;
+            if (stride[i] == p.D || rows == 1) {
+                copy(dst, from, rows * p.D * uint32_t(sizeof(T)), bars + 8 * s);
+            } else {
+                for (int r = 0; r < rows; ++r)
+                    copy(dst + r * p.D * uint32_t(sizeof(T)), from + r * stride[i], p.D * uint32_t(sizeof(T)), bars + 8 * s);
+            }
+        }
+        next += int64_t(gridDim.x) * slots;
+    }
+    __device__ __forceinline__ void arrive() {           // the rows of this turn are in their buffer
+        const Waiter wait = {dead, p.status};
+        wait(bars + 8 * stage, turn & 1);
+    }
+    template <int E>
+    __device__ __forceinline__ void read(int i, int slot, int gt, int G, float (&x)[E]) const {
+        const T *s = reinterpret_cast<const T *>(mem + (size_t(stage) * INPUTS + i) * bytes) + slot * p.D;
+        constexpr int VEC = Elem<T>::VEC;
+#pragma unroll
+        for (int j = 0; j < E; j += VEC) {
+            uint4 r = make_uint4(0, 0, 0, 0);
+            const int e = element<T, true>(j, gt, G);
+            if (e < p.D) r = *reinterpret_cast<const uint4 *>(s + e);
+            Elem<T>::unpack(r, x + j);
+        }
+    }
+    __device__ __forceinline__ void release() {          // everybody has read: ask for the rows that come here next
+        __syncthreads();
+        if (threadIdx.x == 0) issue(stage);
+        if (++stage == p.stages) {
+            stage = 0;
+            ++turn;
+        }
+    }
+};
+
+template <class T, bool ALIGNED, int E>
+__device__ __forceinline__ void load_weight(const void *w, int dtype, int gt, int G, int D, float missing, float (&x)[E]) {
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+        const int e = element<T, ALIGNED>(i, gt, G);
         x[i] = w && e < D ? load_as_float(w, dtype, e) : missing;
     }
 }
 
 // Sum over the G threads of a row: lanes by shuffles (G <= 32: a power of two), warps through shared memory.  Two
 // halves of `red` are used in turn, so one barrier a reduction suffices.
-template <int N>
-__device__ __forceinline__ void row_sum(float (&v)[N], int G, int warps, float *red, int &turn) {
-    const int top = G < 32 ? G : 32;
-#pragma unroll
-    for (int j = 0; j < N; ++j)
-        for (int d = top / 2; d; d /= 2) v[j] += __shfl_xor_sync(~0u, v[j], d);
-    if (G <= 32) return;
-    const int warp = threadIdx.x >> 5, first = warp / (G / 32) * (G / 32);
-    float *r = red + turn * 2 * 32;
-    turn ^= 1;
-    if ((threadIdx.x & 31) == 0)
-#pragma unroll
-        for (int j = 0; j < N; ++j) r[j * 32 + warp] = v[j];
-    __syncthreads();
-#pragma unroll
-    for (int j = 0; j < N; ++j) {
-        float s = 0.f;
-        for (int w = 0; w < G / 32; ++w) s += r[j * 32 + first + w];
-        v[j] = s;
+struct RowSum {
+    float *red;
+    int lanes, first, warps, turn;       // lanes of a warp in one sum; the row's first warp and their number (0: one warp)
+    __device__ __forceinline__ RowSum(float *shared, int G) : red(shared), lanes(G < 32 ? G : 32), warps(G > 32 ? G / 32 : 0), turn(0) {
+        first = warps ? int(threadIdx.x >> 5) / warps * warps : 0;
     }
-}
+    template <int N>
+    __device__ __forceinline__ void operator()(float (&v)[N]) {
+        if (lanes == 32) {
+#pragma unroll
+            for (int d = 16; d; d /= 2)
+#pragma unroll
+                for (int j = 0; j < N; ++j) v[j] += __shfl_xor_sync(~0u, v[j], d);
+        } else {
+            for (int d = lanes / 2; d; d /= 2)
+#pragma unroll
+                for (int j = 0; j < N; ++j) v[j] += __shfl_xor_sync(~0u, v[j], d);
+        }
+        if (warps == 0) return;
+        float *r = red + turn * 2 * 32;
+        turn ^= 1;
+        if ((threadIdx.x & 31) == 0)
+#pragma unroll
+            for (int j = 0; j < N; ++j) r[j * 32 + (threadIdx.x >> 5)] = v[j];
+        __syncthreads();
+        r += first;
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            float s = 0.f;
+            if ((warps & 7) == 0) {
+                for (int w = 0; w < warps; w += 8) {
+                    const float4 a = *reinterpret_cast<const float4 *>(r + j * 32 + w), b = *reinterpret_cast<const float4 *>(r + j * 32 + w + 4);
+                    s += ((a.x + a.y) + (a.z + a.w)) + ((b.x + b.y) + (b.z + b.w));
+                }
+            } else {
+                for (int w = 0; w < warps; ++w) s += r[j * 32 + w];
+            }
+            v[j] = s;
+        }
+    }
+};
 
-__device__ __forceinline__ float gate_value(float z, int act, float &slope) {
+// The gates' values in place of the gates, and their slopes: s c with c = 1 or z, and s ((1 - s) c + 0 or 1).
+template <bool SLOPE, int E>
+__device__ __forceinline__ void open_gates(float (&z)[E], float (&slope)[E], int act) {
     if (act == ACT_NONE) {
-        slope = 1.f;
-        return z;
+#pragma unroll
+        for (int i = 0; i < E; ++i) slope[i] = 1.f;
+        return;
     }
-    const float s = 1.f / (1.f + expf(-z));
-    if (act == ACT_SIGMOID) {
-        slope = s * (1.f - s);
-        return s;
+    const bool silu = act == ACT_SILU;
+    const float one = silu ? 1.f : 0.f;
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+        // 1 / (1 + 2^(-z log2 e)), each part good to a few 2^-24: two slow instructions an element, where the exact
+        // exponential and division took half of a kernel's time.  Past |z| = 88 it is 0 and 1.
+        float e, s;
+        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(z[i] * -1.4426950408889634f));
+        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(s) : "f"(1.f + e));
+        const float c = silu ? z[i] : 1.f;
+        if (SLOPE) slope[i] = s * fmaf(1.f - s, c, one);
+        z[i] = s * c;
     }
-    slope = s * (1.f + z * (1.f - s));
-    return z * s;
 }
 
-template <class T, bool ALIGNED>
-__global__ void __launch_bounds__(NORM_THREADS) norm_forward_kernel(NormParams p) {
-    __shared__ float red[2 * 2 * 32];
+// E = 8: up to 256 threads, three CTAs an SM; E = 16, for long rows: a thread's work outside of its elements (addresses,
+// barriers, reductions) was half of all at eight.
+template <class T, bool ALIGNED, bool RING, int E>
+__global__ void __launch_bounds__(E == 8 ? 256 : 512, E == 8 ? 3 : 1) norm_forward_kernel(const __grid_constant__ NormParams p) {
+    extern __shared__ __align__(128) unsigned char dynamic[];
+    __shared__ __align__(16) float red[2 * 2 * 32];
+    __shared__ uint64_t bar[8];
+    __shared__ int gave_up;
     const int G = p.groups, slots = blockDim.x / G, gt = threadIdx.x % G, slot = threadIdx.x / G;
     const float inv_d = 1.f / float(p.D);
-    int turn = 0;
-    float pw[EPT], sc[EPT], qw[EPT];
-    load_weight<ALIGNED>(p.post_w, p.w_dtype, gt, G, p.D, 1.f, pw);
-    load_weight<ALIGNED>(p.scale, p.w_dtype, gt, G, p.D, p.scale_value, sc);
-    load_weight<ALIGNED>(p.pre_w, p.w_dtype, gt, G, p.D, 1.f, qw);
+    RowSum row_sum(red, G);
+    RowRing<T, 3> ring(p, dynamic, bar, &gave_up, slots);
+    if (RING) {
+        ring.src[0] = p.x; ring.src[1] = p.residual; ring.src[2] = p.gate;
+        ring.stride[0] = p.x_s; ring.stride[1] = p.r_s; ring.stride[2] = p.g_s;
+        ring.init();
+    }
+    float w[E], qw[E];                                // w: scale and post_weight in one
+    load_weight<T, ALIGNED>(p.post_w, p.w_dtype, gt, G, p.D, 1.f, w);
+    load_weight<T, ALIGNED>(p.scale, p.w_dtype, gt, G, p.D, p.scale_value, qw);
+#pragma unroll
+    for (int i = 0; i < E; ++i) w[i] *= qw[i];
+    load_weight<T, ALIGNED>(p.pre_w, p.w_dtype, gt, G, p.D, 1.f, qw);
     for (int64_t first = int64_t(blockIdx.x) * slots; first < p.rows; first += int64_t(gridDim.x) * slots) {
         const int64_t row = first + slot;
         const bool live = row < p.rows;
-        float x[EPT] = {}, r[EPT] = {}, z[EPT] = {};
-        if (live) {
+        float x[E] = {}, r[E] = {}, z[E] = {};
+        if (RING) {
+            ring.arrive();
+            if (live) {
+                ring.read(0, slot, gt, G, x);
+                if (p.residual) ring.read(1, slot, gt, G, r);
+                if (p.gate) ring.read(2, slot, gt, G, z);
+            }
+            ring.release();
+        } else if (live) {
             load_row<T, ALIGNED>(p.x, row * p.x_s, gt, G, p.D, x);
             if (p.residual) load_row<T, ALIGNED>(p.residual, row * p.r_s, gt, G, p.D, r);
             if (p.gate) load_row<T, ALIGNED>(p.gate, row * p.g_s, gt, G, p.D, z);
@@ -185,25 +324,28 @@ __global__ void __launch_bounds__(NORM_THREADS) norm_forward_kernel(NormParams p
         if (p.post_w) {
             float s[1] = {};
 #pragma unroll
-            for (int i = 0; i < EPT; ++i) s[0] += x[i] * x[i];
-            row_sum(s, G, blockDim.x / 32, red, turn);
+            for (int i = 0; i < E; ++i) s[0] += x[i] * x[i];
+            row_sum(s);
             rx = rsqrtf(s[0] * inv_d + p.eps);
         }
+        if (p.gate) {
+            float none[E];
+            open_gates<false>(z, none, p.act);
 #pragma unroll
-        for (int i = 0; i < EPT; ++i) {
-            float slope, a = 1.f;
-            if (p.gate) a = gate_value(z[i], p.act, slope);
-            r[i] += sc[i] * (a * (x[i] * rx * pw[i]));
+            for (int i = 0; i < E; ++i) r[i] += w[i] * (z[i] * (x[i] * rx));
+        } else {
+#pragma unroll
+            for (int i = 0; i < E; ++i) r[i] += w[i] * (x[i] * rx);
         }
         if (live) store_row<T, ALIGNED>(p.hidden, row * p.D, gt, G, p.D, r);
         if (p.pre_w) {
             float s[1] = {};
 #pragma unroll
-            for (int i = 0; i < EPT; ++i) s[0] += r[i] * r[i];
-            row_sum(s, G, blockDim.x / 32, red, turn);
+            for (int i = 0; i < E; ++i) s[0] += r[i] * r[i];
+            row_sum(s);
             const float rh = rsqrtf(s[0] * inv_d + p.eps);
 #pragma unroll
-            for (int i = 0; i < EPT; ++i) r[i] *= rh * qw[i];
+            for (int i = 0; i < E; ++i) r[i] *= rh * qw[i];
             if (live) store_row<T, ALIGNED>(p.normed, row * p.D, gt, G, p.D, r);
         }
     }
@@ -211,20 +353,31 @@ __global__ void __launch_bounds__(NORM_THREADS) norm_forward_kernel(NormParams p
 
 // WIDE: rows whose threads have only 64 registers each.  The weights are read where they are used (from the L1 cache) and
 // their gradients are summed in shared memory, by the thread that owns the element.
-template <class T, bool ALIGNED, bool WIDE>
-__global__ void __launch_bounds__(WIDE ? NORM_THREADS : NORM_NARROW) norm_backward_kernel(NormParams p) {
-    extern __shared__ float sums[];                       // [slots][3][D] when rows share a CTA; WIDE: [3][EPT][threads]
-    __shared__ float red[2 * 2 * 32];
+template <class T, bool ALIGNED, bool WIDE, bool RING>
+__global__ void __launch_bounds__(WIDE ? NORM_THREADS : NORM_NARROW) norm_backward_kernel(const __grid_constant__ NormParams p) {
+    extern __shared__ __align__(128) unsigned char dynamic[];
+    float *sums = reinterpret_cast<float *>(dynamic);     // [slots][3][D] when rows share a CTA; WIDE: [3][EPT][threads]
+    __shared__ __align__(16) float red[2 * 2 * 32];
+    __shared__ uint64_t bar[8];
+    __shared__ int gave_up;
+    constexpr int EPT = 8;
     const int G = p.groups, slots = blockDim.x / G, gt = threadIdx.x % G, slot = threadIdx.x / G;
     const float inv_d = 1.f / float(p.D);
-    int turn = 0;
+    RowSum row_sum(red, G);
     float pw[EPT], sc[EPT], qw[EPT], d_w[WIDE ? 1 : 3][EPT] = {};
     if (!WIDE) {
-        load_weight<ALIGNED>(p.post_w, p.w_dtype, gt, G, p.D, 1.f, pw);
-        load_weight<ALIGNED>(p.scale, p.w_dtype, gt, G, p.D, p.scale_value, sc);
-        load_weight<ALIGNED>(p.pre_w, p.w_dtype, gt, G, p.D, 1.f, qw);
+        load_weight<T, ALIGNED>(p.post_w, p.w_dtype, gt, G, p.D, 1.f, pw);
+        load_weight<T, ALIGNED>(p.scale, p.w_dtype, gt, G, p.D, p.scale_value, sc);
+        load_weight<T, ALIGNED>(p.pre_w, p.w_dtype, gt, G, p.D, 1.f, qw);
     } else if (p.partial) {
         for (int i = 0; i < 3 * EPT; ++i) sums[i * blockDim.x + threadIdx.x] = 0.f;
+    }
+    // the ring lies behind the sums where these are kept from the start, and in their place else
+    RowRing<T, 5> ring(p, dynamic + (WIDE && p.partial ? 3 * EPT * blockDim.x * 4 : 0), bar, &gave_up, slots);
+    if (RING) {
+        ring.src[0] = p.x; ring.src[1] = p.residual; ring.src[2] = p.gate; ring.src[3] = p.d_hidden; ring.src[4] = p.d_normed;
+        ring.stride[0] = p.x_s; ring.stride[1] = p.r_s; ring.stride[2] = p.g_s; ring.stride[3] = p.dh_s; ring.stride[4] = p.dy_s;
+        ring.init();
     }
     const auto add = [&](int which, int i, float x) {     // post, scale, pre
         if (!WIDE) d_w[WIDE ? 0 : which][i] += x;
@@ -234,7 +387,17 @@ __global__ void __launch_bounds__(WIDE ? NORM_THREADS : NORM_NARROW) norm_backwa
         const int64_t row = first + slot;
         const bool live = row < p.rows;
         float x[EPT] = {}, h[EPT] = {}, z[EPT] = {}, dh[EPT] = {}, dy[EPT] = {};
-        if (live) {
+        if (RING) {
+            ring.arrive();
+            if (live) {
+                ring.read(0, slot, gt, G, x);
+                if (p.residual) ring.read(1, slot, gt, G, h);
+                if (p.gate) ring.read(2, slot, gt, G, z);
+                if (p.d_hidden) ring.read(3, slot, gt, G, dh);
+                if (p.d_normed) ring.read(4, slot, gt, G, dy);
+            }
+            ring.release();
+        } else if (live) {
             load_row<T, ALIGNED>(p.x, row * p.x_s, gt, G, p.D, x);
             if (p.residual) load_row<T, ALIGNED>(p.residual, row * p.r_s, gt, G, p.D, h);
             if (p.gate) load_row<T, ALIGNED>(p.gate, row * p.g_s, gt, G, p.D, z);
@@ -246,30 +409,37 @@ __global__ void __launch_bounds__(WIDE ? NORM_THREADS : NORM_NARROW) norm_backwa
             float s[1] = {};
 #pragma unroll
             for (int i = 0; i < EPT; ++i) s[0] += x[i] * x[i];
-            row_sum(s, G, blockDim.x / 32, red, turn);
+            row_sum(s);
             rx = rsqrtf(s[0] * inv_d + p.eps);
         }
         if (WIDE) {
-            load_weight<ALIGNED>(p.post_w, p.w_dtype, gt, G, p.D, 1.f, pw);
-            load_weight<ALIGNED>(p.scale, p.w_dtype, gt, G, p.D, p.scale_value, sc);
+            load_weight<T, ALIGNED>(p.post_w, p.w_dtype, gt, G, p.D, 1.f, pw);
+            load_weight<T, ALIGNED>(p.scale, p.w_dtype, gt, G, p.D, p.scale_value, sc);
         }
         float slope[EPT];
+        if (p.gate) {
+            open_gates<true>(z, slope, p.act);                            // from here on the gate's value
+        } else {
+#pragma unroll
+            for (int i = 0; i < EPT; ++i) {
+                z[i] = 1.f;
+                slope[i] = 0.f;
+            }
+        }
 #pragma unroll
         for (int i = 0; i < EPT; ++i) {
-            slope[i] = 0.f;
-            z[i] = p.gate ? gate_value(z[i], p.act, slope[i]) : 1.f;      // from here on the gate's value
             x[i] *= rx;                                                   // ... and the normed x
             h[i] += sc[i] * (z[i] * (x[i] * pw[i]));
         }
         if (p.d_normed) {
-            if (WIDE) load_weight<ALIGNED>(p.pre_w, p.w_dtype, gt, G, p.D, 1.f, qw);
+            if (WIDE) load_weight<T, ALIGNED>(p.pre_w, p.w_dtype, gt, G, p.D, 1.f, qw);
             float s[2] = {};
 #pragma unroll
             for (int i = 0; i < EPT; ++i) {
                 s[0] += h[i] * h[i];
                 s[1] += dy[i] * qw[i] * h[i];
             }
-            row_sum(s, G, blockDim.x / 32, red, turn);
+            row_sum(s);
             const float rh = rsqrtf(s[0] * inv_d + p.eps), c = s[1] * rh * rh * inv_d;
 #pragma unroll
             for (int i = 0; i < EPT; ++i) {
@@ -279,8 +449,8 @@ __global__ void __launch_bounds__(WIDE ? NORM_THREADS : NORM_NARROW) norm_backwa
         }
         if (p.d_residual && live) store_row<T, ALIGNED>(p.d_residual, row * p.D, gt, G, p.D, dh);
         if (WIDE) {
-            load_weight<ALIGNED>(p.post_w, p.w_dtype, gt, G, p.D, 1.f, pw);
-            load_weight<ALIGNED>(p.scale, p.w_dtype, gt, G, p.D, p.scale_value, sc);
+            load_weight<T, ALIGNED>(p.post_w, p.w_dtype, gt, G, p.D, 1.f, pw);
+            load_weight<T, ALIGNED>(p.scale, p.w_dtype, gt, G, p.D, p.scale_value, sc);
         }
 #pragma unroll
         for (int i = 0; i < EPT; ++i) {
@@ -298,7 +468,7 @@ __global__ void __launch_bounds__(WIDE ? NORM_THREADS : NORM_NARROW) norm_backwa
                 dh[i] *= pw[i];
                 s[0] += dh[i] * x[i];
             }
-            row_sum(s, G, blockDim.x / 32, red, turn);
+            row_sum(s);
             const float c = s[0] * inv_d;
 #pragma unroll
             for (int i = 0; i < EPT; ++i) dh[i] = rx * (dh[i] - x[i] * c);
@@ -306,10 +476,11 @@ __global__ void __launch_bounds__(WIDE ? NORM_THREADS : NORM_NARROW) norm_backwa
         if (live) store_row<T, ALIGNED>(p.d_x, row * p.D, gt, G, p.D, dh);
     }
     if (!p.partial) return;
+    if (RING && slots > 1) __syncthreads();               // the sums take the ring's place
     float *to = p.partial + int64_t(blockIdx.x) * 3 * p.D;
 #pragma unroll
     for (int i = 0; i < EPT; ++i) {
-        const int e = element<ALIGNED>(i, gt, G);
+        const int e = element<T, ALIGNED>(i, gt, G);
         if (e >= p.D) continue;
 #pragma unroll
         for (int w = 0; w < 3; ++w) {
@@ -348,9 +519,9 @@ __global__ void __launch_bounds__(1024) norm_weights_kernel(const float *partial
     }
 }
 
-// Threads of a row: eight elements each; below a warp a power of two, so that several rows share one.
-static void norm_shape(int D, int *groups, int *threads) {
-    int need = (D + EPT - 1) / EPT, g = 1;
+// Threads of a row: E elements each; below a warp a power of two, so that several rows share one.
+static void norm_shape(int D, int E, int *groups, int *threads) {
+    int need = (D + E - 1) / E, g = 1;
     if (need <= 32) {
         while (g < need) g *= 2;
     } else {
@@ -360,11 +531,11 @@ static void norm_shape(int D, int *groups, int *threads) {
     *threads = g >= 256 ? g : 256 / g * g;
 }
 
-// CTAs: what the SMs hold at once by registers (128 a thread in the backward, 64 in the forward); every CTA walks rows
-// with its weights in registers.
-static int norm_grid(int64_t rows, int groups, int threads, int sms, bool backward) {
+// CTAs: what the SMs hold at once by registers (128 a thread, 80 in the forward of short rows); every CTA walks rows with
+// its weights in registers.
+static int norm_grid(int64_t rows, int groups, int threads, int sms, bool short_forward) {
     const int64_t slots = threads / groups, need = (rows + slots - 1) / slots;
-    const int per_sm = (backward ? NORM_NARROW : 1024) / threads;
+    const int per_sm = (short_forward ? 768 : 512) / threads;
     const int64_t most = int64_t(sms) * (per_sm > 1 ? per_sm : 1);
     return static_cast<int>(need < most ? need : most);
 }
@@ -385,37 +556,61 @@ static int norm_device(int *sms) {
     return ASCAN_OK;
 }
 
-template <class T, bool ALIGNED, bool WIDE>
-static int launch_norm_back(const NormParams &p, int grid, int threads, cudaStream_t st) {
-    const int slots = threads / p.groups;
-    size_t smem = 0;
-    if (p.partial) smem = WIDE ? size_t(3) * EPT * threads * 4 : slots > 1 ? size_t(slots) * 3 * p.D * 4 : 0;   // at most 96 KB
-    if (WIDE && cudaFuncSetAttribute(norm_backward_kernel<T, ALIGNED, WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                     3 * EPT * NORM_THREADS * 4) != cudaSuccess)
+// Stages of the ring: at most four, in what two CTAs of an SM share (the long rows' kernels, one or two CTAs an SM) or
+// three; none where two do not fit, or where no CTA comes to a second turn.  `kept`: bytes of the sums that live beside it.
+static int ring_stages(const NormParams &p, int inputs, int slots, int grid, bool short_forward, size_t size, size_t kept) {
+    const size_t buffer = size_t(inputs) * slots * p.D * size, room = short_forward ? 48 * 1024 : 104 * 1024;
+    if (p.rows <= int64_t(grid) * slots) return 0;
+    int n = 4;
+    while (n > 1 && kept + n * buffer > room) --n;
+    if (n == 1 && !short_forward && kept + 2 * buffer <= 216 * 1024) n = 2;
+    return n > 1 ? n : 0;
+}
+
+template <class K>
+static int launch_norm(K kernel, const NormParams &p, int grid, int threads, size_t smem, cudaStream_t st) {
+    if (smem > 40 * 1024 && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)) != cudaSuccess)
         return ASCAN_ERR_LAUNCH;
-    norm_backward_kernel<T, ALIGNED, WIDE><<<grid, threads, smem, st>>>(p);
+    kernel<<<grid, threads, smem, st>>>(p);
     return cudaGetLastError() == cudaSuccess ? ASCAN_OK : ASCAN_ERR_LAUNCH;
 }
 
-template <class T, bool ALIGNED>
-static int launch_norm_kernel(const NormParams &p, int grid, int threads, bool backward, cudaStream_t st) {
-    if (backward)
-        return threads > NORM_NARROW ? launch_norm_back<T, ALIGNED, true>(p, grid, threads, st)
-                                     : launch_norm_back<T, ALIGNED, false>(p, grid, threads, st);
-    norm_forward_kernel<T, ALIGNED><<<grid, threads, 0, st>>>(p);
-    return cudaGetLastError() == cudaSuccess ? ASCAN_OK : ASCAN_ERR_LAUNCH;
+template <class T, bool ALIGNED, bool WIDE>
+static int launch_back(NormParams p, int grid, int threads, cudaStream_t st) {
+    const int slots = threads / p.groups;
+    size_t sums = 0;
+    if (p.partial) sums = WIDE ? size_t(3) * 8 * threads * 4 : slots > 1 ? size_t(slots) * 3 * p.D * 4 : 0;   // at most 96 KB
+    p.stages = ALIGNED ? ring_stages(p, 5, slots, grid, false, sizeof(T), WIDE ? sums : 0) : 0;
+    const size_t ring = size_t(p.stages) * 5 * slots * p.D * sizeof(T);
+    const size_t smem = WIDE ? sums + ring : sums > ring ? sums : ring;
+    if (ALIGNED && p.stages) return launch_norm(norm_backward_kernel<T, ALIGNED, WIDE, ALIGNED>, p, grid, threads, smem, st);
+    return launch_norm(norm_backward_kernel<T, ALIGNED, WIDE, false>, p, grid, threads, smem, st);
+}
+
+template <class T, bool ALIGNED, int E>
+static int launch_fore(NormParams p, int grid, int threads, cudaStream_t st) {
+    const int slots = threads / p.groups;
+    p.stages = ALIGNED ? ring_stages(p, 3, slots, grid, E == 8, sizeof(T), 0) : 0;
+    const size_t smem = size_t(p.stages) * 3 * slots * p.D * sizeof(T);
+    if (ALIGNED && p.stages) return launch_norm(norm_forward_kernel<T, ALIGNED, ALIGNED, E>, p, grid, threads, smem, st);
+    return launch_norm(norm_forward_kernel<T, ALIGNED, false, E>, p, grid, threads, smem, st);
 }
 
 template <class T>
-static int launch_norm_type(const NormParams &p, int grid, int threads, bool aligned, bool backward, cudaStream_t st) {
-    return aligned ? launch_norm_kernel<T, true>(p, grid, threads, backward, st)
-                   : launch_norm_kernel<T, false>(p, grid, threads, backward, st);
+static int launch_type(const NormParams &p, int grid, int threads, bool aligned, bool backward, cudaStream_t st) {
+    if (backward) {
+        if (threads > NORM_NARROW)
+            return aligned ? launch_back<T, true, true>(p, grid, threads, st) : launch_back<T, false, true>(p, grid, threads, st);
+        return aligned ? launch_back<T, true, false>(p, grid, threads, st) : launch_back<T, false, false>(p, grid, threads, st);
+    }
+    if (p.D > 1024) return aligned ? launch_fore<T, true, 16>(p, grid, threads, st) : launch_fore<T, false, 16>(p, grid, threads, st);
+    return aligned ? launch_fore<T, true, 8>(p, grid, threads, st) : launch_fore<T, false, 8>(p, grid, threads, st);
 }
 
-static int launch_norm(const NormParams &p, int dtype, int grid, int threads, bool aligned, bool backward, cudaStream_t st) {
-    if (dtype == ASCAN_F32) return launch_norm_type<float>(p, grid, threads, aligned, backward, st);
-    if (dtype == ASCAN_BF16) return launch_norm_type<bf16>(p, grid, threads, aligned, backward, st);
-    return launch_norm_type<__half>(p, grid, threads, aligned, backward, st);
+static int launch_norm_by_type(const NormParams &p, int dtype, int grid, int threads, bool aligned, bool backward, cudaStream_t st) {
+    if (dtype == ASCAN_F32) return launch_type<float>(p, grid, threads, aligned, backward, st);
+    if (dtype == ASCAN_BF16) return launch_type<bf16>(p, grid, threads, aligned, backward, st);
+    return launch_type<__half>(p, grid, threads, aligned, backward, st);
 }
 
 static int norm_fill(const ascan_norm *a, NormParams &p, bool *aligned) {
@@ -438,6 +633,7 @@ static int norm_fill(const ascan_norm *a, NormParams &p, bool *aligned) {
     p.post_w = a->post_weight;
     p.scale = a->scale;
     p.pre_w = a->pre_weight;
+    p.status = a->status;
     const int vec = a->dtype == ASCAN_F32 ? 4 : 8;
     const auto ok = [&](const void *q, int64_t s) { return !q || ((reinterpret_cast<uintptr_t>(q) & 15) == 0 && s % vec == 0); };
     *aligned = a->dim % vec == 0 && ok(p.x, p.x_s) && ok(p.residual, p.r_s) && ok(p.gate, p.g_s);
@@ -464,8 +660,8 @@ int ascan_norm_forward(const ascan_norm *a, void *hidden, void *normed, void *st
     aligned = aligned && on16(hidden) && on16(normed);
     int sms = 0, threads;
     if ((rc = norm_device(&sms)) != ASCAN_OK) return rc;
-    norm_shape(p.D, &p.groups, &threads);
-    return launch_norm(p, a->dtype, norm_grid(p.rows, p.groups, threads, sms, false), threads, aligned, false,
+    norm_shape(p.D, p.D > 1024 ? 16 : 8, &p.groups, &threads);
+    return launch_norm_by_type(p, a->dtype, norm_grid(p.rows, p.groups, threads, sms, p.D <= 1024), threads, aligned, false,
                        static_cast<cudaStream_t>(stream));
 }
 
@@ -478,8 +674,8 @@ size_t ascan_norm_backward_bytes(const ascan_norm *a) {
         cudaGetLastError();
         sms = 148;          // no device to ask: size for a full B200
     }
-    norm_shape(p.D, &p.groups, &threads);
-    return size_t(norm_grid(p.rows, p.groups, threads, sms, true)) * 3 * p.D * 4;
+    norm_shape(p.D, 8, &p.groups, &threads);
+    return size_t(norm_grid(p.rows, p.groups, threads, sms, false)) * 3 * p.D * 4;
 }
 
 int ascan_norm_backward(const ascan_norm *a, const void *d_hidden, int64_t d_hidden_stride, const void *d_normed, int64_t d_normed_stride,
@@ -505,10 +701,10 @@ int ascan_norm_backward(const ascan_norm *a, const void *d_hidden, int64_t d_hid
               (!d_hidden || d_hidden_stride % vec == 0) && (!d_normed || d_normed_stride % vec == 0);
     int sms = 0, threads;
     if ((rc = norm_device(&sms)) != ASCAN_OK) return rc;
-    norm_shape(p.D, &p.groups, &threads);
-    const int grid = norm_grid(p.rows, p.groups, threads, sms, true);
+    norm_shape(p.D, 8, &p.groups, &threads);
+    const int grid = norm_grid(p.rows, p.groups, threads, sms, false);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (p.rows > 0 && (rc = launch_norm(p, a->dtype, grid, threads, aligned, true, st)) != ASCAN_OK) return rc;
+    if (p.rows > 0 && (rc = launch_norm_by_type(p, a->dtype, grid, threads, aligned, true, st)) != ASCAN_OK) return rc;
     if (weights) {         // without rows: zeros
         norm_weights_kernel<<<dim3((p.D + 31) / 32, 3), 1024, 0, st>>>(p.partial, p.rows > 0 ? grid : 0, p.D, p.w_dtype, d_post_weight,
                                                                        d_scale, d_pre_weight);

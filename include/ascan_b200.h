@@ -407,6 +407,7 @@ typedef struct {
     int32_t heads_k, heads, k_dim, v_dim;
     int32_t dtype, log_gates_dtype, betas_dtype;
     float scale;
+    int *status;                                   /* as in ascan_delta                       */
 } ascan_delta_token;
 int ascan_delta_step(const ascan_delta_token *args, void *out, float *state, int64_t pool, int64_t slot_stride,
                      const void *slots, int slots_64, void *stream);
@@ -425,6 +426,7 @@ typedef struct {
     int64_t rows, x_stride, residual_stride, gate_stride;
     int32_t dim, dtype, weights_dtype, activation;
     float eps, scale_value;
+    int *status;                                   /* as in ascan_delta                       */
 } ascan_norm;
 int ascan_norm_forward(const ascan_norm *args, void *hidden, void *normed, void *stream);
 

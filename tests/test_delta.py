@@ -375,7 +375,7 @@ def state_off(got, want, before, values):
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
 @pytest.mark.parametrize("shape", [(1, 1, 1, 128, 128), (3, 2, 4, 64, 64), (5, 1, 3, 61, 20), (2, 1, 1, 1, 1), (4, 2, 2, 128, 33),
-                                   (70, 2, 8, 128, 128), (2, 1, 2, 100, 1000)])
+                                   (70, 2, 8, 128, 128), (2, 1, 2, 100, 1000), (40, 4, 16, 72, 80), (1030, 1, 1, 16, 16)])
 def test_step(cuda_device, shape, dtype):
     """out: its own rounding, and like the state fp32 sums over K of up to 128 terms: 8 * 2^-24 of what goes in."""
     B, Hk, H, K, V = shape
@@ -397,8 +397,9 @@ def test_step(cuda_device, shape, dtype):
 
 
 @pytest.mark.gpu
-def test_step_padded_rows_and_bad_slots(cuda_device):
-    B, H = 6, 2
+@pytest.mark.parametrize("H", [2, 128])                    # few states, and more than the SMs hold at once
+def test_step_padded_rows_and_bad_slots(cuda_device, H):
+    B = 6
     args = token_inputs(1, B, 1, H, 64, 64, torch.bfloat16, cuda_device)
     pool = torch.randn(4, H, 64, 64, device=cuda_device)
     state = pool.clone()
