@@ -150,7 +150,7 @@ static void fill_back(const ascan_delta *a, DeltaParams &p, Bump &bump, const vo
     const int nt = terms(a->dtype), kp = p.Kp <= 64 ? 64 : 128;
     p.dS = bump.take<__nv_bfloat16>(each * nt * p.Vp * kp);
     p.z = bump.take<__nv_bfloat16>(each * nt * 64 * p.Vp);
-    take_chunks(p, bump);
+    if (!tensor_core_path(a)) take_chunks(p, bump);
     plan_pack(a, d_out, d_out_stride, a->heads, a->v_dim, &p.d_out, bump, jobs, n_jobs);
 }
 
@@ -549,6 +549,10 @@ int ascan_delta_backward(const ascan_delta *a, const void *d_out, const int64_t 
     p.d_b = d_betas;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if ((rc = run_packs(a, jobs, n, st)) != ASCAN_OK) return rc;
+    if (tensor_core_path(a)) {
+        if ((rc = delta_launch_back_sweep_tc(p, st)) != ASCAN_OK) return rc;
+        return delta_launch_grads(p, terms(a->dtype), st);
+    }
     if ((rc = delta_launch_prep(p, terms(a->dtype), st)) != ASCAN_OK) return rc;
     if ((rc = delta_launch_back_sweep(p, terms(a->dtype), sms, st)) != ASCAN_OK) return rc;
     return delta_launch_grads(p, terms(a->dtype), st);

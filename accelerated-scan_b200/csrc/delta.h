@@ -60,6 +60,7 @@ int delta_launch_pack(const void *src, int dtype, const int64_t *strides, int64_
 int delta_launch_prep(const DeltaParams &p, int nt, cudaStream_t st);
 int delta_launch_sweep(const DeltaParams &p, int nt, bool save, int sm_count, cudaStream_t st);
 int delta_launch_sweep_tc(const DeltaParams &p, bool save, cudaStream_t st);
+int delta_launch_back_sweep_tc(const DeltaParams &p, cudaStream_t st);
 int delta_launch_back_sweep(const DeltaParams &p, int nt, int sm_count, cudaStream_t st);
 int delta_launch_grads(const DeltaParams &p, int nt, cudaStream_t st);
 
