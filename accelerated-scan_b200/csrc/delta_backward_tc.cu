@@ -18,7 +18,7 @@ template <int KP>
 __global__ void __launch_bounds__(TC_THREADS, 1) delta_back_sweep_tc_kernel(const __grid_constant__ DeltaParams p,
                                                                             const __grid_constant__ TcMaps maps) {
     extern __shared__ unsigned char smem_raw[];
-    typedef TcLayout<KP, 2> L;
+    typedef TcLayout<KP, true> L;
     typedef TcBackward F;
     constexpr int HK = KP / 2;                         // columns of the state a thread holds
     const TcBlock k = tc_begin<L>(p, smem_raw, 4, 4);
@@ -203,7 +203,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) delta_back_sweep_tc_kernel(cons
 #pragma unroll 1
             for (int turn = 0; turn < sq.chunks; ++turn) {
                 const uint32_t tile = base + ring.stage * L::STAGE, rows = tile_low(tile), down = tile_low(tile, 16384);
-                const uint32_t m = tile_low(base + L::MP + (turn & 1) * L::MP_BYTES), d_out = tile_low(tile + L::KQ_BYTES, 8192);
+                const uint32_t m = tile_low(base + L::M + (turn & 1) * M_BYTES), pt = tile_low(base + L::P + (turn & 1) * L::P_BYTES);
+                const uint32_t d_out = tile_low(tile + L::KQ_BYTES, 8192);
                 // tokens 16 t .. 16 t + 15 reach the tokens up to 16 t + 15 only; the last ones come first and write all
                 k.wait(k.bar(B_PREP + (turn & 1)), (turn >> 1) & 1);
                 if (turn > 0) k.wait(k.bar(B_S), (turn - 1) & 1);          // A1's reader has ended
@@ -212,7 +213,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) delta_back_sweep_tc_kernel(cons
                 for (int t = 3; t >= 0; --t)
 #pragma unroll
                     for (int lo = 0; lo < 2; ++lo)
-                        tc_mma_ss(tmem + F::D2, d_out + ((2048 * t) >> 4), m + ((L::P + 8192 * lo + 2048 * t) >> 4),
+                        tc_mma_ss(tmem + F::D2, d_out + ((2048 * t) >> 4), pt + ((8192 * lo + 2048 * t) >> 4),
                                   mma_desc(16 * (t + 1), true, false, true), t < 3 || lo > 0);
                 tc_commit(k.bar(B_D2));
                 k.wait(k.bar(B_AS), turn & 1);
@@ -233,6 +234,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) delta_back_sweep_tc_kernel(cons
                     tc_mma_ts(tmem + F::D3, tmem + F::DU + 8 * t, m + (8192 >> 4) + at, desc, true);
                 }
                 tc_commit(k.bar(B_D3));
+                ring.m_read(k, turn);
                 k.wait(k.bar(B_A1), turn & 1);
                 tc_fence_after();
 #pragma unroll
@@ -249,7 +251,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) delta_back_sweep_tc_kernel(cons
                     for (int lo = 0; lo < 2; ++lo)
                         tc_mma_ts(tmem + F::S, tmem + F::D1 + 32 * lo + 8 * t, down + kq(0, 16 * t), mma_desc(KP, true, true), true);
                 tc_commit(k.bar(B_S));
-                ring.next(k, turn);
+                ring.next(k);
             }
         }
     } else if (warp == 17) {
@@ -267,7 +269,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) delta_back_sweep_tc_kernel(cons
 template <int KP>
 static int launch_back_sweep_tc(const DeltaParams &p, const TcMaps &maps, cudaStream_t st) {
     const int64_t grid = int64_t(p.n_seqs) * p.H * ((p.Vp + 127) / 128);
-    const int smem = TcLayout<KP, 2>::BYTES;
+    const int smem = TcLayout<KP, true>::BYTES;
     if (grid > 0x7fffffff) return ASCAN_ERR_UNSUPPORTED;
     if (cudaFuncSetAttribute(delta_back_sweep_tc_kernel<KP>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
         return ASCAN_ERR_LAUNCH;

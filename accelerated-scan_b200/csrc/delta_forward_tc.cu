@@ -23,7 +23,7 @@ template <int KP, bool SAVE>
 __global__ void __launch_bounds__(TC_THREADS, 1) delta_sweep_tc_kernel(const __grid_constant__ DeltaParams p,
                                                                        const __grid_constant__ TcMaps maps) {
     extern __shared__ unsigned char smem_raw[];
-    typedef TcLayout<KP, 1> L;
+    typedef TcLayout<KP, false> L;
     typedef TcForward F;
     constexpr int HK = KP / 2;                         // columns of the state a thread holds
     const TcBlock k = tc_begin<L>(p, smem_raw, 4, 5);
@@ -224,7 +224,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) delta_sweep_tc_kernel(const __g
 #pragma unroll
                 for (int s = 0; s < KP / 16; ++s)
                     tc_mma_ts(tmem + F::O1, state_term<HK>(tmem + F::S, s, 0), rows + kq(s, 64), mma_desc(64, false), s > 0);
-                const uint32_t mp = base + L::MP + (c & 1) * L::MP_BYTES, m = tile_low(mp);
+                const uint32_t m = tile_low(base + L::M + (c & 1) * M_BYTES), pt = tile_low(base + L::P + stage * L::P_BYTES);
                 k.wait(k.bar(B_PREP + (c & 1)), (c >> 1) & 1);
                 k.wait(k.bar(B_BX), c & 1);
                 tc_fence_after();
@@ -237,6 +237,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) delta_sweep_tc_kernel(const __g
                     tc_mma_ts(d, tmem + F::BX + 8 * t, m + (8192 >> 4) + at, desc, true);
                 }
                 tc_commit(k.bar(B_D2));
+                ring.m_read(k, c);
                 k.wait(k.bar(B_U), c & 1);
                 tc_fence_after();
 #pragma unroll
@@ -251,10 +252,10 @@ __global__ void __launch_bounds__(TC_THREADS, 1) delta_sweep_tc_kernel(const __g
                 for (int t = 0; t < 4; ++t)
 #pragma unroll
                     for (int lo = 0; lo < 2; ++lo)
-                        tc_mma_ts(tmem + F::O2 + 16 * t, tmem + F::BX + 32 * lo + 8 * t, m + ((L::P + 16 * t * 128 + 32 * t) >> 4),
+                        tc_mma_ts(tmem + F::O2 + 16 * t, tmem + F::BX + 32 * lo + 8 * t, pt + ((16 * t * 128 + 32 * t) >> 4),
                                   mma_desc(64 - 16 * t, false), t + lo > 0);
                 tc_commit(k.bar(B_O));
-                ring.next(k, c);
+                ring.next(k);
             }
         }
     } else if (warp == 17) {
@@ -281,7 +282,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) delta_sweep_tc_kernel(const __g
 template <int KP, bool SAVE>
 static int launch_sweep_tc(const DeltaParams &p, const TcMaps &maps, cudaStream_t st) {
     const int64_t grid = int64_t(p.n_seqs) * p.H * ((p.Vp + 127) / 128);
-    const int smem = TcLayout<KP, 1>::BYTES;
+    const int smem = TcLayout<KP, false>::BYTES;
     if (grid > 0x7fffffff) return ASCAN_ERR_UNSUPPORTED;
     if (cudaFuncSetAttribute(delta_sweep_tc_kernel<KP, SAVE>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
         return ASCAN_ERR_LAUNCH;

@@ -267,7 +267,7 @@ __device__ __forceinline__ void chunk_gates(const float (&g)[2], const float (&b
     const double last = __shfl_sync(~0u, s, 31), end = __shfl_sync(~0u, s, lane | 7), first = __shfl_sync(~0u, G0, lane & ~7);
     const int all = __shfl_sync(~0u, r, 31), r_end = __shfl_sync(~0u, r, lane | 7), r_first = __shfl_sync(~0u, R0, lane & ~7);
     bool plain = r_first == r_end;
-#pragma unroll
+#pragma unroll 1
     for (int j = 0; j < 2; ++j) {
         const int i = 2 * lane + j;
         const double G = j ? s : G0;
@@ -275,18 +275,18 @@ __device__ __forceinline__ void chunk_gates(const float (&g)[2], const float (&b
         const float hi = float(G), gam = R == 0 ? expf(hi) : 0.f, back = float(first - G);
         sc[SC_GAM * 64 + i] = gam;
         sc[SC_OUT * 64 + i] = scale * gam;
-        const float gam_c = R == all ? expf(float(last - G)) : 0.f;
+        const float be = j ? beta[1] : beta[0], gam_c = R == all ? expf(float(last - G)) : 0.f;
         sc[SC_GAMC * 64 + i] = gam_c;
-        sc[SC_GAMC_BETA * 64 + i] = gam_c * beta[j];
-        sc[SC_BETA * 64 + i] = beta[j];
+        sc[SC_GAMC_BETA * 64 + i] = gam_c * be;
+        sc[SC_BETA * 64 + i] = be;
         sc[SC_GHI * 64 + i] = hi;
         sc[SC_GLO * 64 + i] = float(G - double(hi));
         sc[SC_RESET * 64 + i] = float(R);
         const float to_end = R == r_end ? expf(float(end - G)) : 0.f, to_first = expf(back);
         gs.w[0][0][i] = to_end;
         gs.w[0][1][i] = to_first;
-        gs.w[1][0][i] = to_end * beta[j];
-        gs.w[1][1][i] = to_first * beta[j];
+        gs.w[1][0][i] = to_end * be;
+        gs.w[1][1][i] = to_first * be;
         plain = plain && fabsf(back) <= 60.f;
     }
     const unsigned ok = __ballot_sync(~0u, plain);
@@ -299,7 +299,7 @@ __device__ __forceinline__ void chunk_gates(const float (&g)[2], const float (&b
 __device__ __forceinline__ void row_factors(float (&f)[4][128], float factor, const GateShared &gs, int i, int tid) {
     const float *sc = gs.sc;
     const int bi = i >> 4;
-#pragma unroll
+#pragma unroll 1
     for (int bj = 0; bj < 4; ++bj) {
         const int ref = bj == bi ? 16 * bj : 16 * bj + 15;
         f[bj][tid] = bj > bi ? 0.f : factor * decay_between(sc[SC_GHI * 64 + i], sc[SC_GLO * 64 + i], sc[SC_RESET * 64 + i],

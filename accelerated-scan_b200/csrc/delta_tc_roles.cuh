@@ -88,19 +88,20 @@ static inline int make_store_map(TcMaps *maps, void *dst, const DeltaParams &p, 
     return make_map(&maps->out, out, p, p.V, p.H, swizzled ? 64 : 128, swizzled);
 }
 
-// Shared memory: three stages of tiles ([K; Q] as 128 rows, one block of 64 columns or two; V or d_out), two buffers of what
-// a chunk's preparation yields, three of its gates.  P has P_TERMS tiles.
-template <int KP, int P_TERMS>
+// Shared memory: three stages of tiles ([K; Q] as 128 rows, one block of 64 columns or two; V or d_out), two buffers of M, two
+// or three of P, three of the gates.  The forward reads a chunk's P last, so P has a third buffer there: the next preparation
+// but one then waits for M's reader only.  The backward reads P first.
+template <int KP, bool BACK>
 struct TcLayout {
     static constexpr int HALVES = KP / 64, KQ_BYTES = HALVES * 16384, V_BYTES = 64 * 256, STAGE = KQ_BYTES + V_BYTES;
-    static constexpr int MP = 3 * STAGE, P = M_BYTES, MP_BYTES = M_BYTES + P_TERMS * 8192;       // M (hi, lo), P
-    static constexpr int SC = MP + 2 * MP_BYTES, PREP = SC + 3 * sizeof(GateShared);
+    static constexpr int M = 3 * STAGE, P = M + 2 * M_BYTES, P_BYTES = (BACK ? 2 : 1) * 8192, P_BUFFERS = BACK ? 2 : 3;
+    static constexpr int SC = P + P_BUFFERS * P_BYTES, PREP = SC + 3 * sizeof(GateShared);
     static constexpr int BARS = PREP + 2 * 4 * 128 * 4, BYTES = BARS + 256 + 1024;               // and 1024 to align the start
     static constexpr int KK = 448;           // columns of tensor memory of [K; Q] K^T
 };
-static_assert(TcLayout<128, 2>::BYTES <= 227 * 1024, "shared memory");
+static_assert(TcLayout<128, false>::BYTES <= 227 * 1024 && TcLayout<128, true>::BYTES <= 227 * 1024, "shared memory");
 
-// Barriers: filled tiles, prepared chunks, gates; commits of K K^T and of a preparation's last reader; K K^T read; tile free
+// Barriers: filled tiles, prepared chunks, gates; commits of K K^T and of M's reader; K K^T read; tile free
 // (the commit of its last product and eight warps); a sequence's last tile.  From B_OWN on each kernel's.
 enum : int { B_TILE = 0, B_PREP = 3, B_GATES = 5, B_KK = 8, B_MP = 10, B_KREAD = 12, B_FREE = 13, B_TAIL = 16, B_OWN = 17 };
 
@@ -158,8 +159,7 @@ __device__ __forceinline__ void tc_end(const TcBlock &k) {
 template <class L, bool BACK>
 __device__ __forceinline__ void prepare_chunks(const DeltaParams &p, const TcBlock &k) {
     const int t = threadIdx.x & 127, lane = t & 31, pw = t >> 5, team = threadIdx.x >> 7 & 1;
-    unsigned char *mp = k.smem + L::MP + team * L::MP_BYTES;
-    float *m = reinterpret_cast<float *>(mp);
+    float *m = reinterpret_cast<float *>(k.smem + L::M + team * M_BYTES);
     auto &f = reinterpret_cast<float (*)[4][128]>(k.smem + L::PREP)[team];
     const auto sync = [&] { asm volatile("bar.sync %0, 128;" :: "r"(2 + team) : "memory"); };
     const int i = t & 63;
@@ -169,6 +169,7 @@ __device__ __forceinline__ void prepare_chunks(const DeltaParams &p, const TcBlo
     for (int turn = team; turn < k.sq.chunks; turn += 2) {
         const GateShared &gs = reinterpret_cast<const GateShared *>(k.smem + L::SC)[turn % 3];
         k.wait(k.bar(B_GATES + turn % 3), (turn / 3) & 1);
+        unsigned char *pt = k.smem + L::P + turn % L::P_BUFFERS * L::P_BYTES;      // three: free when this chunk's gates were written
         const float factor = !l_row ? p.scale : BACK ? gs.sc[SC_BETA * 64 + i] : 1.f;
         row_factors(f, factor, gs, i, t);
         if (turn >= 2) k.wait(k.bar(B_MP + team), ((turn - 2) >> 1) & 1);
@@ -188,9 +189,9 @@ __device__ __forceinline__ void prepare_chunks(const DeltaParams &p, const TcBlo
                         if (BACK) split2(x[8 * pc + 2 * j], x[8 * pc + 2 * j + 1], hi[j], lo[j]);
                         else hi[j] = pack2(x[8 * pc + 2 * j], x[8 * pc + 2 * j + 1]);
                     }
-                    *reinterpret_cast<uint4 *>(mp + L::P + tile_off<8>(i, 2 * bj + pc)) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                    *reinterpret_cast<uint4 *>(pt + tile_off<8>(i, 2 * bj + pc)) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
                     if (BACK)
-                        *reinterpret_cast<uint4 *>(mp + L::P + 8192 + tile_off<8>(i, 2 * bj + pc)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                        *reinterpret_cast<uint4 *>(pt + 8192 + tile_off<8>(i, 2 * bj + pc)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
                 }
             }
         });
@@ -297,9 +298,9 @@ struct TileRing {
             issue_kk<L>(k, c, c);
         }
     }
-    __device__ __forceinline__ void next(const TcBlock &k, int turn) {
+    // Where M's reader has been issued: the group that prepared this chunk is free for the next but one.
+    __device__ __forceinline__ void m_read(const TcBlock &k, int turn) {
         tc_commit(k.bar(B_MP + (turn & 1)));
-        tc_commit(k.bar(B_FREE + stage));
         if (turn + 2 < k.sq.chunks) {
             k.wait(k.bar(B_TILE + ahead), ahead_turn & 1);
             k.wait(k.bar(B_KREAD), (turn + 1) & 1);
@@ -310,6 +311,9 @@ struct TileRing {
             ahead = 0;
             ++ahead_turn;
         }
+    }
+    __device__ __forceinline__ void next(const TcBlock &k) {
+        tc_commit(k.bar(B_FREE + stage));
         if (++stage == 3) stage = 0;
     }
 };
