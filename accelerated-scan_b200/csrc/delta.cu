@@ -35,7 +35,7 @@ static int check_shape(const ascan_delta *a) {
     if (a->k_dim > 128 || a->v_dim > 1024 || a->heads > 65535) return ASCAN_ERR_UNSUPPORTED;
     const int64_t slots = a->n_seqs ? a->seqlen / DELTA_CHUNK + a->n_seqs : a->batch * ((a->seqlen + 63) / DELTA_CHUNK);
     const int64_t chains = (a->n_seqs ? a->n_seqs : a->batch) * int64_t(a->heads) * ((a->v_dim + 15) / 16);
-    if (slots > 0x7fffffff || chains > 0x7fffffff) return ASCAN_ERR_UNSUPPORTED;
+    if (slots > 0x7fffffff / a->heads || chains > 0x7fffffff || a->seqlen > (int64_t(1) << 30)) return ASCAN_ERR_UNSUPPORTED;
     return ASCAN_OK;
 }
 
@@ -549,9 +549,10 @@ int ascan_delta_backward(const ascan_delta *a, const void *d_out, const int64_t 
     p.d_b = d_betas;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if ((rc = run_packs(a, jobs, n, st)) != ASCAN_OK) return rc;
+    if ((rc = delta_launch_zero_outside(p, st)) != ASCAN_OK) return rc;
     if (tensor_core_path(a)) {
         if ((rc = delta_launch_back_sweep_tc(p, st)) != ASCAN_OK) return rc;
-        return delta_launch_grads(p, terms(a->dtype), st);
+        return p.Kp > 64 ? delta_launch_grads_tc(p, sms, st) : delta_launch_grads(p, terms(a->dtype), st);
     }
     if ((rc = delta_launch_prep(p, terms(a->dtype), st)) != ASCAN_OK) return rc;
     if ((rc = delta_launch_back_sweep(p, terms(a->dtype), sms, st)) != ASCAN_OK) return rc;

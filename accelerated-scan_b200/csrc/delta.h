@@ -62,6 +62,8 @@ int delta_launch_sweep(const DeltaParams &p, int nt, bool save, int sm_count, cu
 int delta_launch_sweep_tc(const DeltaParams &p, bool save, cudaStream_t st);
 int delta_launch_back_sweep_tc(const DeltaParams &p, cudaStream_t st);
 int delta_launch_back_sweep(const DeltaParams &p, int nt, int sm_count, cudaStream_t st);
+int delta_launch_zero_outside(const DeltaParams &p, cudaStream_t st);
 int delta_launch_grads(const DeltaParams &p, int nt, cudaStream_t st);
+int delta_launch_grads_tc(const DeltaParams &p, int sm_count, cudaStream_t st);
 
 }  // namespace ascan

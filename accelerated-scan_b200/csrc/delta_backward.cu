@@ -655,12 +655,14 @@ static int launch_grads_nt(const DeltaParams &p, int nt, cudaStream_t st) {
     return nt == 1 ? launch_grads<KP, 1, true>(p, st) : launch_grads<KP, 2, true>(p, st);
 }
 
+int delta_launch_zero_outside(const DeltaParams &p, cudaStream_t st) {
+    if (!p.packed) return ASCAN_OK;
+    delta_zero_outside_kernel<<<64, 256, 0, st>>>(p);
+    return cudaGetLastError() == cudaSuccess ? ASCAN_OK : ASCAN_ERR_LAUNCH;
+}
+
 int delta_launch_grads(const DeltaParams &p, int nt, cudaStream_t st) {
     if (p.slots == 0) return ASCAN_OK;
-    if (p.packed) {
-        delta_zero_outside_kernel<<<64, 256, 0, st>>>(p);
-        if (cudaGetLastError() != cudaSuccess) return ASCAN_ERR_LAUNCH;
-    }
     return p.Kp <= 64 ? launch_grads_nt<64>(p, nt, st) : launch_grads_nt<128>(p, nt, st);
 }
 

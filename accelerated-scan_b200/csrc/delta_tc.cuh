@@ -104,6 +104,9 @@ __device__ __forceinline__ void tmem_ld16(uint32_t (&r)[16], uint32_t a) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
                  : ASCAN_R8(r, 0), ASCAN_R8(r, 8) : "r"(a));
 }
+__device__ __forceinline__ void tmem_ld8(uint32_t (&r)[8], uint32_t a) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];" : ASCAN_R8(r, 0) : "r"(a));
+}
 __device__ __forceinline__ void tmem_st32(uint32_t a, const uint32_t (&r)[32]) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,"
                  "%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};"

@@ -12,8 +12,10 @@ struct TcMaps {
     bool store;                // out can be written by copies: rows start on 16 bytes
 };
 
-// (column, head, token, batch) of planes; a box is `cols` columns of 64 tokens.  What lies outside of the array reads as zero.
-static inline int make_map(CUtensorMap *map, const Planes &x, const DeltaParams &p, int d, int heads, int cols, bool swizzled) {
+// (column, head, token, batch) of planes, in boxes of `cols` columns, `box_heads` heads and `tokens` tokens.  What lies outside
+// of the array reads as zero.
+static inline int make_box_map(CUtensorMap *map, const Planes &x, const DeltaParams &p, int d, int heads, int cols, int box_heads,
+                               int tokens, bool swizzled) {
     typedef CUresult (*Encode)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
                                const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
                                CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
@@ -32,7 +34,7 @@ static inline int make_map(CUtensorMap *map, const Planes &x, const DeltaParams 
     const cuuint64_t dims[4] = {cuuint64_t(d), cuuint64_t(heads), cuuint64_t(p.T), cuuint64_t(p.batch)};
     const cuuint64_t strides[3] = {cuuint64_t(heads > 1 ? x.sh : d) * 2, cuuint64_t(p.T > 1 ? x.st : int64_t(heads) * d) * 2,
                                    cuuint64_t(p.batch > 1 ? x.sb : p.T * heads * d) * 2};
-    const cuuint32_t box[4] = {cuuint32_t(cols), 1, 64, 1}, unit[4] = {1, 1, 1, 1};
+    const cuuint32_t box[4] = {cuuint32_t(cols), cuuint32_t(box_heads), cuuint32_t(tokens), 1}, unit[4] = {1, 1, 1, 1};
     const auto run = [&] {
         return encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<__nv_bfloat16 *>(x.p), dims, strides, box, unit,
                       CU_TENSOR_MAP_INTERLEAVE_NONE, swizzled ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
@@ -45,6 +47,9 @@ static inline int make_map(CUtensorMap *map, const Planes &x, const DeltaParams 
         rc = run();
     }
     return rc == CUDA_SUCCESS ? ASCAN_OK : ASCAN_ERR_LAUNCH;
+}
+static inline int make_map(CUtensorMap *map, const Planes &x, const DeltaParams &p, int d, int heads, int cols, bool swizzled) {
+    return make_box_map(map, x, p, d, heads, cols, 1, 64, swizzled);
 }
 
 // The next chunk's log gates and rates, two tokens a lane, held as they are until they are needed: a conversion would wait
