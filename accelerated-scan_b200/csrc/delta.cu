@@ -35,7 +35,7 @@ static int check_shape(const ascan_delta *a) {
     if (a->k_dim > 128 || a->v_dim > 1024 || a->heads > 65535) return ASCAN_ERR_UNSUPPORTED;
     const int64_t slots = a->n_seqs ? a->seqlen / DELTA_CHUNK + a->n_seqs : a->batch * ((a->seqlen + 63) / DELTA_CHUNK);
     const int64_t chains = (a->n_seqs ? a->n_seqs : a->batch) * int64_t(a->heads) * ((a->v_dim + 15) / 16);
-    if (slots > 0x7fffffff / a->heads || chains > 0x7fffffff || a->seqlen > (int64_t(1) << 30)) return ASCAN_ERR_UNSUPPORTED;
+    if (slots > 0x3fffffff / a->heads || chains > 0x7fffffff || a->seqlen > (int64_t(1) << 30)) return ASCAN_ERR_UNSUPPORTED;
     return ASCAN_OK;
 }
 
@@ -137,7 +137,7 @@ static void fill(const ascan_delta *a, DeltaParams &p, Bump &bump, bool keep, Pa
     if (keep) {
         const int nt = terms(a->dtype), kp = p.Kp <= 64 ? 64 : 128;
         p.S = bump.take<__nv_bfloat16>(each * nt * p.Vp * kp);
-        p.e = bump.take<__nv_bfloat16>(each * nt * 64 * p.Vp);
+        p.e = bump.take<__nv_bfloat16>(each * 2 * 64 * p.Vp);
     }
     p.status = a->status;
 }
@@ -149,7 +149,7 @@ static void fill_back(const ascan_delta *a, DeltaParams &p, Bump &bump, const vo
     const int64_t each = int64_t(p.slots) * p.H;
     const int nt = terms(a->dtype), kp = p.Kp <= 64 ? 64 : 128;
     p.dS = bump.take<__nv_bfloat16>(each * nt * p.Vp * kp);
-    p.z = bump.take<__nv_bfloat16>(each * nt * 64 * p.Vp);
+    p.z = bump.take<__nv_bfloat16>(each * 2 * 64 * p.Vp);
     if (!tensor_core_path(a)) take_chunks(p, bump);
     plan_pack(a, d_out, d_out_stride, a->heads, a->v_dim, &p.d_out, bump, jobs, n_jobs);
 }
@@ -516,8 +516,8 @@ int ascan_delta_forward(const ascan_delta *a, void *out, float *final_state, int
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if ((rc = run_packs(a, jobs, n, st)) != ASCAN_OK) return rc;
     if (tensor_core_path(a)) return delta_launch_sweep_tc(p, keep != 0, st);
-    if ((rc = delta_launch_prep(p, terms(a->dtype), st)) != ASCAN_OK) return rc;
-    return delta_launch_sweep(p, terms(a->dtype), keep != 0, sms, st);
+    if ((rc = delta_launch_prep(p, st)) != ASCAN_OK) return rc;
+    return delta_launch_sweep(p, keep != 0, sms, st);
 }
 
 int ascan_delta_backward(const ascan_delta *a, const void *d_out, const int64_t *d_out_stride, const float *d_final_state,
@@ -552,11 +552,11 @@ int ascan_delta_backward(const ascan_delta *a, const void *d_out, const int64_t 
     if ((rc = delta_launch_zero_outside(p, st)) != ASCAN_OK) return rc;
     if (tensor_core_path(a)) {
         if ((rc = delta_launch_back_sweep_tc(p, st)) != ASCAN_OK) return rc;
-        return p.Kp > 64 ? delta_launch_grads_tc(p, sms, st) : delta_launch_grads(p, terms(a->dtype), st);
+        return delta_launch_grads_tc(p, sms, st);
     }
-    if ((rc = delta_launch_prep(p, terms(a->dtype), st)) != ASCAN_OK) return rc;
-    if ((rc = delta_launch_back_sweep(p, terms(a->dtype), sms, st)) != ASCAN_OK) return rc;
-    return delta_launch_grads(p, terms(a->dtype), st);
+    if ((rc = delta_launch_prep(p, st)) != ASCAN_OK) return rc;
+    if ((rc = delta_launch_back_sweep(p, sms, st)) != ASCAN_OK) return rc;
+    return delta_launch_grads(p, st);
 }
 
 int ascan_delta_step(const ascan_delta_token *a, void *out, float *state, int64_t pool, int64_t slot_stride, const void *slots,

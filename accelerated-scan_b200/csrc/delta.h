@@ -57,13 +57,13 @@ struct DeltaParams {
 
 int delta_launch_pack(const void *src, int dtype, const int64_t *strides, int64_t batch, int64_t T, int heads, int d,
                       int dp, __nv_bfloat16 *dst, int64_t plane, cudaStream_t st);
-int delta_launch_prep(const DeltaParams &p, int nt, cudaStream_t st);
-int delta_launch_sweep(const DeltaParams &p, int nt, bool save, int sm_count, cudaStream_t st);
+int delta_launch_prep(const DeltaParams &p, cudaStream_t st);
+int delta_launch_sweep(const DeltaParams &p, bool save, int sm_count, cudaStream_t st);
 int delta_launch_sweep_tc(const DeltaParams &p, bool save, cudaStream_t st);
 int delta_launch_back_sweep_tc(const DeltaParams &p, cudaStream_t st);
-int delta_launch_back_sweep(const DeltaParams &p, int nt, int sm_count, cudaStream_t st);
+int delta_launch_back_sweep(const DeltaParams &p, int sm_count, cudaStream_t st);
 int delta_launch_zero_outside(const DeltaParams &p, cudaStream_t st);
-int delta_launch_grads(const DeltaParams &p, int nt, cudaStream_t st);
+int delta_launch_grads(const DeltaParams &p, cudaStream_t st);
 int delta_launch_grads_tc(const DeltaParams &p, int sm_count, cudaStream_t st);
 
 }  // namespace ascan

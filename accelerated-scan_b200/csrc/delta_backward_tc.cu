@@ -107,36 +107,32 @@ __global__ void __launch_bounds__(TC_THREADS, 1) delta_back_sweep_tc_kernel(cons
             tc_fence_after();
             tmem_ld32(r, t0 + F::D3 + 32 * part);
             tc_wait_ld();
-            bf16 *z = p.z + ((int64_t(sq.slot0 + c) * p.H + h) * p.Vp + v0 + v) * 64 + 32 * part;
 #pragma unroll
             for (int q = 0; q < 2; ++q) {
-                uint32_t hi[8], lo[8], zb[8];
+                uint32_t hi[8], lo[8];
 #pragma unroll
                 for (int j = 0; j < 8; j += 2) {
                     const int i = 8 * q + j;
                     const ulonglong2 be = scalars(SC_BETA, 2 * i), ga = scalars(SC_GAM, 2 * i);
                     x[i] = add2(x[i], two_bits(r[2 * i], r[2 * i + 1]));
                     x[i + 1] = add2(x[i + 1], two_bits(r[2 * i + 2], r[2 * i + 3]));
-                    zb[j] = pack_f2(x[i]);
-                    zb[j + 1] = pack_f2(x[i + 1]);
-                    x[i] = mul2(be.x, x[i]);
-                    x[i + 1] = mul2(be.y, x[i + 1]);
-                    split_f2(mul2(ga.x, x[i]), hi[j], lo[j]);
-                    split_f2(mul2(ga.y, x[i + 1]), hi[j + 1], lo[j + 1]);
+                    split_f2(mul2(ga.x, mul2(be.x, x[i])), hi[j], lo[j]);
+                    split_f2(mul2(ga.y, mul2(be.y, x[i + 1])), hi[j + 1], lo[j + 1]);
                 }
                 tmem_st8(t0 + F::D1 + 16 * part + 8 * q, hi);
                 tmem_st8(t0 + F::D1 + 32 + 16 * part + 8 * q, lo);
-                if (v0 + v < p.Vp) {
-                    reinterpret_cast<uint4 *>(z)[2 * q] = make_uint4(zb[0], zb[1], zb[2], zb[3]);
-                    reinterpret_cast<uint4 *>(z)[2 * q + 1] = make_uint4(zb[4], zb[5], zb[6], zb[7]);
-                }
             }
             hand_over(k, B_YZ);
+            if (v0 + v < p.Vp)
+                keep_tokens(x, p.z + ((int64_t(sq.slot0 + c) * p.H + h) * 2 * p.Vp + v0 + v) * 64 + 32 * part, int64_t(p.Vp) * 64);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {           // dV in the place of d_out, which nobody needs any more
-                const uint32_t y = pack_f2(x[i]);
+            for (int i = 0; i < 16; i += 2) {        // dV in the place of d_out, which nobody needs any more
+                const ulonglong2 be = scalars(SC_BETA, 2 * i);
+                const uint32_t y = pack_f2(mul2(be.x, x[i])), w = pack_f2(mul2(be.y, x[i + 1]));
                 *element(2 * i) = static_cast<uint16_t>(y);
                 *element(2 * i + 1) = static_cast<uint16_t>(y >> 16);
+                *element(2 * i + 2) = static_cast<uint16_t>(w);
+                *element(2 * i + 3) = static_cast<uint16_t>(w >> 16);
             }
             const int64_t left = sq.len - int64_t(c) * 64;
             const bool by_copy = maps.store && (left >= 64 || sq.t0 + sq.len == p.T);        // as in the forward sweep

@@ -53,11 +53,11 @@ int delta_launch_pack(const void *src, int dtype, const int64_t *strides, int64_
 constexpr int PREP_PITCH = 68;     // floats; rows stay 16-byte aligned
 
 template <int KP>
-constexpr size_t prep_smem(int nt) {
-    return size_t(nt) * 2 * 64 * KP * 2 + 2 * 64 * PREP_PITCH * 4 + 4 * 16 * 20 * 4 + SC_ARRAYS * 64 * 4;
+constexpr size_t prep_smem() {
+    return size_t(4) * 64 * KP * 2 + 2 * 64 * PREP_PITCH * 4 + 4 * 16 * 20 * 4 + SC_ARRAYS * 64 * 4;
 }
 
-template <int KP, int NT>
+template <int KP>
 __global__ void __launch_bounds__(128) delta_prep_kernel(DeltaParams p) {
     extern __shared__ __align__(128) unsigned char smem[];
     constexpr int NCH = KP / 8, TILE = 64 * KP * 2;
@@ -65,11 +65,11 @@ __global__ void __launch_bounds__(128) delta_prep_kernel(DeltaParams p) {
     const int slot = blockIdx.x, hk = blockIdx.y, group = p.H / p.Hk;
     const Chunk ch = get_chunk(p, slot);
     if (ch.rows == 0) return;
-    const uint32_t sk = smem_addr(smem), sq = sk + NT * TILE;
-    float *sL = reinterpret_cast<float *>(smem + 2 * NT * TILE), *sA = sL + 64 * PREP_PITCH, *sD = sA + 64 * PREP_PITCH;
+    const uint32_t sk = smem_addr(smem), sq = sk + 2 * TILE;
+    float *sL = reinterpret_cast<float *>(smem + 4 * TILE), *sA = sL + 64 * PREP_PITCH, *sD = sA + 64 * PREP_PITCH;
     float *ssc = sD + 4 * 16 * 20;
 
-    for (int pl = 0; pl < NT; ++pl) {
+    for (int pl = 0; pl < 2; ++pl) {
         load_tile<NCH>(sk + pl * TILE, p.k.p + pl * p.k.plane + ch.b * p.k.sb + ch.t0 * p.k.st + hk * p.k.sh, p.k.st, ch.rows,
                        p.Kp / 8, tid, 128);
         load_tile<NCH>(sq + pl * TILE, p.q.p + pl * p.q.plane + ch.b * p.q.sb + ch.t0 * p.q.st + hk * p.q.sh, p.q.st, ch.rows,
@@ -83,9 +83,9 @@ __global__ void __launch_bounds__(128) delta_prep_kernel(DeltaParams p) {
     float kk[8][4] = {}, qk[8][4] = {};
 #pragma unroll
     for (int s = 0; s < KP / 16; ++s) {
-        uint32_t ak[NT][4], aq[NT][4];
+        uint32_t ak[2][4], aq[2][4];
 #pragma unroll
-        for (int pl = 0; pl < NT; ++pl) {
+        for (int pl = 0; pl < 2; ++pl) {
             ldsm4(ak[pl], addr_an<NCH>(sk + pl * TILE, 16 * warp, 2 * s, lane));
             ldsm4(aq[pl], addr_an<NCH>(sq + pl * TILE, 16 * warp, 2 * s, lane));
         }
@@ -93,11 +93,11 @@ __global__ void __launch_bounds__(128) delta_prep_kernel(DeltaParams p) {
         for (int np = 0; np < 4; ++np) {
             if (np > warp) break;
 #pragma unroll
-            for (int pl = 0; pl < NT; ++pl) {
+            for (int pl = 0; pl < 2; ++pl) {
                 uint32_t b[4];
                 ldsm4(b, addr_bn<NCH>(sk + pl * TILE, 16 * np, 2 * s, lane));
 #pragma unroll
-                for (int pa = 0; pa + pl < NT; ++pa) {
+                for (int pa = 0; pa < 2; ++pa) {
                     mma(kk[2 * np], ak[pa], b[0], b[1]);
                     mma(kk[2 * np + 1], ak[pa], b[2], b[3]);
                     mma(qk[2 * np], aq[pa], b[0], b[1]);
@@ -261,19 +261,18 @@ __global__ void __launch_bounds__(128) delta_prep_kernel(DeltaParams p) {
     }
 }
 
-template <int KP, int NT>
+template <int KP>
 static int launch_prep(const DeltaParams &p, cudaStream_t st) {
-    const size_t smem = prep_smem<KP>(NT);
-    if (cudaFuncSetAttribute(delta_prep_kernel<KP, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)) != cudaSuccess)
+    const size_t smem = prep_smem<KP>();
+    if (cudaFuncSetAttribute(delta_prep_kernel<KP>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)) != cudaSuccess)
         return ASCAN_ERR_LAUNCH;
-    delta_prep_kernel<KP, NT><<<dim3(p.slots, p.Hk), 128, smem, st>>>(p);
+    delta_prep_kernel<KP><<<dim3(p.slots, p.Hk), 128, smem, st>>>(p);
     return cudaGetLastError() == cudaSuccess ? ASCAN_OK : ASCAN_ERR_LAUNCH;
 }
 
-int delta_launch_prep(const DeltaParams &p, int nt, cudaStream_t st) {
+int delta_launch_prep(const DeltaParams &p, cudaStream_t st) {
     if (p.slots == 0) return ASCAN_OK;
-    if (p.Kp <= 64) return nt == 1 ? launch_prep<64, 1>(p, st) : launch_prep<64, 2>(p, st);
-    return nt == 1 ? launch_prep<128, 1>(p, st) : launch_prep<128, 2>(p, st);
+    return p.Kp <= 64 ? launch_prep<64>(p, st) : launch_prep<128>(p, st);
 }
 
 // ---- forward sweep ---------------------------------------------------------------------------------------------------
@@ -287,25 +286,25 @@ int delta_launch_prep(const DeltaParams &p, int nt, cudaStream_t st) {
 // keeps its precision from chunk to chunk; for bf16 inputs out alone takes S, u and P in one term (2^-8, as its own
 // rounding).  fp16 and fp32 inputs are two planes, and every product takes the three largest of the four term products.
 
-template <int KP, int NT>
+template <int KP>
 struct SweepLayout {
     static constexpr int TILE = 64 * KP * 2;
-    static constexpr int K = 0, Q = NT * TILE, M = 2 * NT * TILE, P = M + 2 * 8192, SC = P + NT * 8192;
+    static constexpr int K = 0, Q = 2 * TILE, M = 4 * TILE, P = M + 2 * 8192, SC = P + 2 * 8192;
     static constexpr int V = SC + SC_ARRAYS * 256;
-    static constexpr int V_WARP = NT * 64 * 32;             // [plane][piece][64] of 16 bytes
-    static constexpr int STAGING = 32 * KP > 2048 * NT ? 32 * KP : 2048 * NT;
+    static constexpr int V_WARP = 2 * 64 * 32;             // [plane][piece][64] of 16 bytes
+    static constexpr int STAGING = 32 * KP > 4096 ? 32 * KP : 4096;
     static constexpr size_t bytes(int warps) { return 2 * (size_t(V) + size_t(warps) * V_WARP) + size_t(warps) * STAGING; }
 };
 
-template <int KP, int NT>
+template <int KP>
 __device__ __forceinline__ void sweep_load(const DeltaParams &p, uint32_t base, const Sequence &sq, int c, int h, int hk, int v0_cta,
                                            int warps, int tid, int threads) {
-    typedef SweepLayout<KP, NT> L;
+    typedef SweepLayout<KP> L;
     const int64_t t0 = sq.t0 + int64_t(c) * 64, left = sq.len - int64_t(c) * 64;
     const int rows = static_cast<int>(left < 64 ? left : 64);
     const int64_t at = int64_t(sq.slot0 + c) * p.H + h;
 #pragma unroll
-    for (int pl = 0; pl < NT; ++pl) {
+    for (int pl = 0; pl < 2; ++pl) {
         load_tile<KP / 8>(base + L::K + pl * L::TILE, p.k.p + pl * p.k.plane + sq.b * p.k.sb + t0 * p.k.st + hk * p.k.sh, p.k.st,
                           rows, p.Kp / 8, tid, threads);
         load_tile<KP / 8>(base + L::Q + pl * L::TILE, p.q.p + pl * p.q.plane + sq.b * p.q.sb + t0 * p.q.st + hk * p.q.sh, p.q.st,
@@ -324,10 +323,10 @@ __device__ __forceinline__ void sweep_load(const DeltaParams &p, uint32_t base, 
     for (int i = tid; i < SC_ARRAYS * 16; i += threads) cp16(base + L::SC + i * 16, p.sc + at * SC_ARRAYS * 64 + i * 4, true);
 }
 
-template <int KP, int NT, bool SAVE>
+template <int KP, bool SAVE>
 __global__ void __launch_bounds__(256, 1) delta_sweep_kernel(DeltaParams p) {
     extern __shared__ __align__(128) unsigned char smem[];
-    typedef SweepLayout<KP, NT> L;
+    typedef SweepLayout<KP> L;
     constexpr int NCH = KP / 8, KT = KP / 8;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, threads = blockDim.x, warps = threads >> 5;
     const int g = lane >> 2, t2 = 2 * (lane & 3);
@@ -351,11 +350,11 @@ __global__ void __launch_bounds__(256, 1) delta_sweep_kernel(DeltaParams p) {
         }
 
     if (sq.chunks > 0) {
-        sweep_load<KP, NT>(p, base, sq, 0, h, hk, v0_cta, warps, tid, threads);
+        sweep_load<KP>(p, base, sq, 0, h, hk, v0_cta, warps, tid, threads);
         cp_commit();
     }
     for (int c = 0; c < sq.chunks; ++c) {
-        if (c + 1 < sq.chunks) sweep_load<KP, NT>(p, base + ((c + 1) & 1) * stage_bytes, sq, c + 1, h, hk, v0_cta, warps, tid, threads);
+        if (c + 1 < sq.chunks) sweep_load<KP>(p, base + ((c + 1) & 1) * stage_bytes, sq, c + 1, h, hk, v0_cta, warps, tid, threads);
         cp_commit();
         cp_wait<1>();
         __syncthreads();
@@ -364,7 +363,7 @@ __global__ void __launch_bounds__(256, 1) delta_sweep_kernel(DeltaParams p) {
         const int64_t at = int64_t(sq.slot0 + c) * p.H + h;
         const int64_t left = sq.len - int64_t(c) * 64;
         const int rows = static_cast<int>(left < 64 ? left : 64);
-        if (SAVE) save_state<KP, NT>(stg, stg_p, s, p.S + at * NT * p.Vp * KP, v0, p.Vp, lane);
+        if (SAVE) save_state<KP>(stg, stg_p, s, p.S + at * 2 * p.Vp * KP, v0, p.Vp, lane);
 
         float x[8][4] = {}, o[8][4] = {};
 #pragma unroll
@@ -381,21 +380,17 @@ __global__ void __launch_bounds__(256, 1) delta_sweep_kernel(DeltaParams p) {
                 mma(x[2 * np + 1], a[0], b[2], b[3]);
                 mma(x[2 * np], a[1], b[0], b[1]);
                 mma(x[2 * np + 1], a[1], b[2], b[3]);
-                if (NT == 2) {
-                    ldsm4(b, addr_bn<NCH>(st + L::K + L::TILE, 16 * np, 2 * kk, lane));
-                    mma(x[2 * np], a[0], b[0], b[1]);
-                    mma(x[2 * np + 1], a[0], b[2], b[3]);
-                }
+                ldsm4(b, addr_bn<NCH>(st + L::K + L::TILE, 16 * np, 2 * kk, lane));
+                mma(x[2 * np], a[0], b[0], b[1]);
+                mma(x[2 * np + 1], a[0], b[2], b[3]);
                 ldsm4(b, addr_bn<NCH>(st + L::Q, 16 * np, 2 * kk, lane));
                 mma(o[2 * np], a[0], b[0], b[1]);
                 mma(o[2 * np + 1], a[0], b[2], b[3]);
-                if (NT == 2) {
-                    mma(o[2 * np], a[1], b[0], b[1]);
-                    mma(o[2 * np + 1], a[1], b[2], b[3]);
-                    ldsm4(b, addr_bn<NCH>(st + L::Q + L::TILE, 16 * np, 2 * kk, lane));
-                    mma(o[2 * np], a[0], b[0], b[1]);
-                    mma(o[2 * np + 1], a[0], b[2], b[3]);
-                }
+                mma(o[2 * np], a[1], b[0], b[1]);
+                mma(o[2 * np + 1], a[1], b[2], b[3]);
+                ldsm4(b, addr_bn<NCH>(st + L::Q + L::TILE, 16 * np, 2 * kk, lane));
+                mma(o[2 * np], a[0], b[0], b[1]);
+                mma(o[2 * np + 1], a[0], b[2], b[3]);
             }
         }
         // x = V - gam (K S0);  out so far scale gam (Q S0)
@@ -403,7 +398,7 @@ __global__ void __launch_bounds__(256, 1) delta_sweep_kernel(DeltaParams p) {
         for (int np = 0; np < 4; ++np) {
             float v[2][4] = {};
 #pragma unroll
-            for (int pl = 0; pl < NT; ++pl) {
+            for (int pl = 0; pl < 2; ++pl) {
                 uint32_t r[4];
                 const int m = lane >> 3;
                 ldsm4t(r, st + L::V + warp * L::V_WARP + ((pl * 2 + (m & 1)) * 64 + 16 * np + (m >> 1) * 8 + (lane & 7)) * 16);
@@ -449,7 +444,7 @@ __global__ void __launch_bounds__(256, 1) delta_sweep_kernel(DeltaParams p) {
                 mma(x[2 * np + 1], a[0], b[2], b[3]);
             }
         }
-        if (SAVE) save_state<64, NT>(stg, stg_p, x, p.e + at * NT * 64 * p.Vp, v0, p.Vp, lane);
+        if (SAVE) save_state<64>(stg, stg_p, x, p.e + at * 2 * 64 * p.Vp, v0, p.Vp, lane);
         const float gam_c = sc[SC_GAM * 64 + 63];
 #pragma unroll
         for (int n = 0; n < KT; ++n)
@@ -476,13 +471,13 @@ __global__ void __launch_bounds__(256, 1) delta_sweep_kernel(DeltaParams p) {
                 ldsm4(b, addr_bn<8>(st + L::P, 16 * np, 2 * kk, lane));
                 mma(o[2 * np], au[0], b[0], b[1]);
                 mma(o[2 * np + 1], au[0], b[2], b[3]);
-                if (NT == 2) {
-                    mma(o[2 * np], au[1], b[0], b[1]);
-                    mma(o[2 * np + 1], au[1], b[2], b[3]);
-                    ldsm4(b, addr_bn<8>(st + L::P + 8192, 16 * np, 2 * kk, lane));
-                    mma(o[2 * np], au[0], b[0], b[1]);
-                    mma(o[2 * np + 1], au[0], b[2], b[3]);
-                }
+                mma(o[2 * np], au[1], b[0], b[1]);
+                mma(o[2 * np + 1], au[1], b[2], b[3]);
+                ldsm4(b, addr_bn<8>(st + L::P + 8192, 16 * np, 2 * kk, lane));
+                mma(o[2 * np], au[0], b[0], b[1]);
+                mma(o[2 * np + 1], au[0], b[2], b[3]);
+                mma(o[2 * np], au[1], b[0], b[1]);
+                mma(o[2 * np + 1], au[1], b[2], b[3]);
             }
 #pragma unroll
             for (int np = 0; np < KP / 16; ++np) {
@@ -492,17 +487,15 @@ __global__ void __launch_bounds__(256, 1) delta_sweep_kernel(DeltaParams p) {
                 mma(s[2 * np + 1], as[0], b[2], b[3]);
                 mma(s[2 * np], as[1], b[0], b[1]);
                 mma(s[2 * np + 1], as[1], b[2], b[3]);
-                if (NT == 2) {
-                    ldsm4t(b, addr_bt<NCH>(st + L::K + L::TILE, 16 * kk, 2 * np, lane));
-                    mma(s[2 * np], as[0], b[0], b[1]);
-                    mma(s[2 * np + 1], as[0], b[2], b[3]);
-                }
+                ldsm4t(b, addr_bt<NCH>(st + L::K + L::TILE, 16 * kk, 2 * np, lane));
+                mma(s[2 * np], as[0], b[0], b[1]);
+                mma(s[2 * np + 1], as[0], b[2], b[3]);
             }
         }
-        stage_transposed<NT>(stg, stg_p, o, lane);
+        stage_transposed(stg, stg_p, o, lane);
         __syncwarp();
         const int64_t t0 = sq.t0 + int64_t(c) * 64;
-        flush_out<NT>(stg_p, p.out, p.dtype, ((sq.b * p.T + t0) * p.H + h) * int64_t(p.V), int64_t(p.H) * p.V, rows, v0, p.V, lane);
+        flush_out(stg_p, p.out, p.dtype, ((sq.b * p.T + t0) * p.H + h) * int64_t(p.V), int64_t(p.H) * p.V, rows, v0, p.V, lane);
         __syncthreads();
     }
     cp_wait<0>();
@@ -524,26 +517,21 @@ __global__ void __launch_bounds__(256, 1) delta_sweep_kernel(DeltaParams p) {
     }
 }
 
-template <int KP, int NT, bool SAVE>
+template <int KP, bool SAVE>
 static int launch_sweep(const DeltaParams &p, int sm_count, cudaStream_t st) {
-    const int warps = sweep_warps(p, sm_count, SweepLayout<KP, NT>::bytes);
-    const size_t smem = SweepLayout<KP, NT>::bytes(warps);
+    const int warps = sweep_warps(p, sm_count, SweepLayout<KP>::bytes);
+    const size_t smem = SweepLayout<KP>::bytes(warps);
     const int64_t grid = int64_t(p.n_seqs) * p.H * ((p.Vp + 16 * warps - 1) / (16 * warps));
     if (grid > 0x7fffffff) return ASCAN_ERR_UNSUPPORTED;
-    if (cudaFuncSetAttribute(delta_sweep_kernel<KP, NT, SAVE>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)) != cudaSuccess)
+    if (cudaFuncSetAttribute(delta_sweep_kernel<KP, SAVE>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)) != cudaSuccess)
         return ASCAN_ERR_LAUNCH;
-    delta_sweep_kernel<KP, NT, SAVE><<<unsigned(grid), 32 * warps, smem, st>>>(p);
+    delta_sweep_kernel<KP, SAVE><<<unsigned(grid), 32 * warps, smem, st>>>(p);
     return cudaGetLastError() == cudaSuccess ? ASCAN_OK : ASCAN_ERR_LAUNCH;
 }
 
-template <int KP>
-static int launch_sweep_nt(const DeltaParams &p, int nt, bool save, int sm_count, cudaStream_t st) {
-    if (nt == 1) return save ? launch_sweep<KP, 1, true>(p, sm_count, st) : launch_sweep<KP, 1, false>(p, sm_count, st);
-    return save ? launch_sweep<KP, 2, true>(p, sm_count, st) : launch_sweep<KP, 2, false>(p, sm_count, st);
-}
-
-int delta_launch_sweep(const DeltaParams &p, int nt, bool save, int sm_count, cudaStream_t st) {
-    return p.Kp <= 64 ? launch_sweep_nt<64>(p, nt, save, sm_count, st) : launch_sweep_nt<128>(p, nt, save, sm_count, st);
+int delta_launch_sweep(const DeltaParams &p, bool save, int sm_count, cudaStream_t st) {
+    if (p.Kp <= 64) return save ? launch_sweep<64, true>(p, sm_count, st) : launch_sweep<64, false>(p, sm_count, st);
+    return save ? launch_sweep<128, true>(p, sm_count, st) : launch_sweep<128, false>(p, sm_count, st);
 }
 
 }  // namespace ascan

@@ -122,13 +122,6 @@ __global__ void __launch_bounds__(TC_THREADS, 1) delta_sweep_tc_kernel(const __g
                 tmem_st8(t0 + F::BX + 32 + 16 * part + 8 * q, lo);
             }
             hand_over(k, B_UO);
-            const int64_t at = int64_t(sq.slot0 + c) * p.H + h;
-            if (SAVE && v0 + v < p.Vp) {
-                uint4 *o = reinterpret_cast<uint4 *>(p.e + (at * p.Vp + v0 + v) * 64 + 32 * part);
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    o[i] = make_uint4(pack_f2(x[4 * i]), pack_f2(x[4 * i + 1]), pack_f2(x[4 * i + 2]), pack_f2(x[4 * i + 3]));
-            }
             const float gam_c = sc[SC_GAM * 64 + 63 - part * 32];
             const f2 gam_c2 = two(gam_c, gam_c);
             k.wait(k.bar(B_S), c & 1);
@@ -144,6 +137,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) delta_sweep_tc_kernel(const __g
                 put_state<HK>(s, t0 + F::S + part * HK, kept(c + 1));
                 hand_over(k, B_AS);
             }
+            if (SAVE && v0 + v < p.Vp)
+                keep_tokens(x, p.e + ((int64_t(sq.slot0 + c) * p.H + h) * 2 * p.Vp + v0 + v) * 64 + 32 * part, int64_t(p.Vp) * 64);
             k.wait(k.bar(B_O), c & 1);
             tc_fence_after();
             uint32_t r2[32];

@@ -1,16 +1,16 @@
-// Gated delta rule, gradients of a chunk on tcgen05: bf16, K in (64, 128].  What delta_backward.cu computes after the sweep,
+// Gated delta rule, gradients of a chunk on tcgen05, for bf16.  What delta_backward.cu computes after the sweep,
 // with every product transposed to 128 rows of K:
 //     dQ^T  = scale gam (S0 d_out^T) + K^T D^T                    D^T[j][i] = scale Gam_ij beta_j (e_j . d_out_i),   i >= j
 //     read^T  = -gam beta (S0 z^T)   + K^T F^T                    F[i][j] = -Gam_ij beta_i beta_j (z_i . e_j),       i > j
 //     write^T = Gam_C beta (dS1 e^T) + Q^T D + K^T F              dbeta_i = z_i . e_i, on F's diagonal
 // All left operands lie in shared memory as they come ([v][k] states, [token][k] keys), D and F serve once by their rows and
-// once by their columns.  D and F are two bf16 terms, everything else is one (of those, e is felt most: dQ and dK are 2.4e-3
-// off, 1.7e-3 of it their own rounding; with one-term D and F 2.9e-3).
+// once by their columns.  D, F, e and z are two bf16 terms, the states one: the gradients are off by little more than their own
+// rounding (1.7e-3; with one-term e and z 2.4e-3 for dQ and dK and 2.9e-3 for dbeta, one-term D and F too 2.9e-3).
 //
 // A persistent CTA walks over (chunk, key head) and the value heads of each; V comes in slabs of 64 through a ring of two, so
 // that copies go on while D, F and the sums are worked on.  16 warps: thread (row, quarter of the columns) holds 16 values of
 // every product.  What bounds it is the chain of an item, products - D, F - products - sums - stores, which one CTA an SM cannot
-// hide: 4 x 4096 tokens, 16 heads of 128 x 128 take 266 us for 470 MB (1.8 TB/s); the mma.sync kernel took 397 there, and 486
+// hide: 4 x 4096 tokens, 16 heads of 128 x 128 take 266 us for 600 MB (2.3 TB/s); the mma.sync kernel took 397 there, and 486
 // went to the first form of this one (8 warps, <S0, dS1> re-read from memory, an exponential an element of D and F).
 #include "delta_tc_roles.cuh"
 
@@ -26,15 +26,15 @@ enum : int { GR_GHI = 0, GR_GLO, GR_RESET, GR_BETA, GR_Q, GR_READ, GR_WRITE, GR_
 
 struct TcGrads {
     static constexpr int TOK = 8192, STATE = 16384;                               // a slab's [64][64] and [64 v][128 k]
-    static constexpr int DO = 0, E = TOK, Z = 2 * TOK, S = 3 * TOK, DS = S + STATE, SLAB = DS + STATE;
-    static constexpr int KQ = 2 * SLAB, KQ_BYTES = 32768;                         // K: two halves of 8 KB, then Q
-    static constexpr int D = KQ + 2 * KQ_BYTES, F = D + 2 * 8192;                 // hi, lo; later dQ and dK on their way out
+    static constexpr int DO = 0, E = TOK, E_LO = 3 * TOK, S = 5 * TOK, DS = S + STATE, SLAB = DS + STATE;    // z behind e
+    static constexpr int KQ = 2 * SLAB, KQ_BYTES = 32768, Z = E + TOK, Z_LO = E_LO + TOK;       // K: two halves of 8 KB, then Q
+    static constexpr int D = KQ + KQ_BYTES, F = D + 2 * 8192;                 // hi, lo; later dQ and dK on their way out
     static constexpr int SC = D + 4 * 8192, RED = SC + GR_ARRAYS * 256, BARS = RED + 1024 + 128, BYTES = BARS + 256 + 1024;
     // columns of tensor memory
     static constexpr int DQ1 = 0, DR1 = 64, DW1 = 128, DP = 192, F0 = 256, DQ2 = 320, DR2 = 384, DW2 = 448;
 };
 static_assert(TcGrads::BYTES <= 227 * 1024, "shared memory");
-enum : int { G_SLAB = 0, G_KQ = 2, G_ACC = 4, G_OUT, G_TAIL, G_DF, G_READ, G_KQ_FREE, G_SLAB_FREE = G_KQ_FREE + 2, G_COUNT = G_SLAB_FREE + 2 };
+enum : int { G_SLAB = 0, G_KQ = 2, G_ACC, G_OUT, G_TAIL, G_DF, G_READ, G_KQ_FREE, G_SLAB_FREE, G_COUNT = G_SLAB_FREE + 2 };
 
 constexpr int GRADS_WARPS = 16, GRADS_COMPUTE = 32 * GRADS_WARPS, GRADS_THREADS = GRADS_COMPUTE + 64;
 
@@ -75,7 +75,7 @@ __global__ void __launch_bounds__(GRADS_THREADS, 1) delta_grads_tc_kernel(const 
             const Chunk ch = get_chunk(p, slot);
             if (ch.rows == 0) continue;
             const int64_t tok0 = ch.b * p.T + ch.t0;
-            const unsigned char *kq = smem + L::KQ + (n_item & 1) * L::KQ_BYTES + (row >> 6) * 8192 + (row & 7) * 2;
+            const unsigned char *kq = smem + L::KQ + (row >> 6) * 8192 + (row & 7) * 2;
             const auto key = [&](int t, int q) {                           // K (Q) of token t, this thread's column
                 return __uint_as_float(uint32_t(*reinterpret_cast<const uint16_t *>(
                     kq + q * 16384 + t * 128 + (((row >> 3 & 7) ^ (t & 7)) << 4))) << 16);
@@ -196,7 +196,7 @@ __global__ void __launch_bounds__(GRADS_THREADS, 1) delta_grads_tc_kernel(const 
                 fence_async_proxy();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(bar(G_DF));
-                if (hh == 0) wait(bar(G_KQ + (n_item & 1)), (n_item >> 1) & 1);
+                if (hh == 0) wait(bar(G_KQ), n_item & 1);
                 wait(bar(G_OUT), n_head & 1);
                 tc_fence_after();
                 float dot[16];
@@ -281,7 +281,7 @@ __global__ void __launch_bounds__(GRADS_THREADS, 1) delta_grads_tc_kernel(const 
                     }
                 }
             }
-            if (lane == 0) mbar_arrive(bar(G_KQ_FREE + (n_item & 1)));
+            if (lane == 0) mbar_arrive(bar(G_KQ_FREE));
             ++n_item;
             // dQ and dK of the key head (the barrier before the sums has seen all their columns)
             for (int i = tid; i < 2 * 64 * 16; i += GRADS_COMPUTE) {
@@ -305,30 +305,7 @@ __global__ void __launch_bounds__(GRADS_THREADS, 1) delta_grads_tc_kernel(const 
             const int slot = static_cast<int>(item / p.Hk), hk = static_cast<int>(item % p.Hk);
             const Chunk ch = get_chunk(p, slot);
             if (ch.rows == 0) continue;
-            const int tok = static_cast<int>(ch.t0), b0 = static_cast<int>(ch.b), buf = n_item & 1;
-            // rows behind a sequence that ends inside the packed row are the next one's: zeros in their place (K and Q only:
-            // of d_out's they reach columns that are not used)
-            const bool tail = ch.rows < 64 && ch.t0 + ch.rows < p.T;
-            if (n_item >= 2) wait(bar(G_KQ_FREE + buf), ((n_item - 2) >> 1) & 1);
-            const uint32_t b = bar(tail ? G_TAIL : G_KQ + buf), dst = base + L::KQ + buf * L::KQ_BYTES;
-            if (lane == 0) {
-                mbar_expect(b, L::KQ_BYTES);
-#pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    tma_load(dst + half * 8192, &maps.k, 64 * half, hk, tok, b0, b);
-                    tma_load(dst + 16384 + half * 8192, &maps.q, 64 * half, hk, tok, b0, b);
-                }
-            }
-            if (tail) {
-                wait(b, n_tail++ & 1);
-                for (int i = lane; i < (64 - ch.rows) * 32; i += 32)
-                    *reinterpret_cast<uint4 *>(smem + L::KQ + buf * L::KQ_BYTES + (i >> 3 & 3) * 8192 + (ch.rows + i / 32) * 128 + (i & 7) * 16) =
-                        make_uint4(0, 0, 0, 0);
-                fence_async_proxy();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(bar(G_KQ + buf));
-            }
-            ++n_item;
+            const int tok = static_cast<int>(ch.t0), b0 = static_cast<int>(ch.b);
             for (int hh = 0; hh < group; ++hh) {
                 const int h = hk * group + hh, at = slot * p.H + h;
                 for (int s = 0; s < slabs; ++s, ++n_slab) {
@@ -338,8 +315,11 @@ __global__ void __launch_bounds__(GRADS_THREADS, 1) delta_grads_tc_kernel(const 
                         const uint32_t d = base + st * L::SLAB, f = bar(G_SLAB + st);
                         mbar_expect(f, L::SLAB);
                         tma_load(d + L::DO, &maps.d_out, 64 * s, h, tok, b0, f);
-                        tma_load(d + L::E, &maps.e, 0, 64 * s, at, 0, f);
-                        tma_load(d + L::Z, &maps.z, 0, 64 * s, at, 0, f);
+#pragma unroll
+                        for (int pl = 0; pl < 2; ++pl) {
+                            tma_load(d + L::E + pl * (L::E_LO - L::E), &maps.e, 0, 64 * s, 2 * at + pl, 0, f);
+                            tma_load(d + L::Z + pl * (L::E_LO - L::E), &maps.z, 0, 64 * s, 2 * at + pl, 0, f);
+                        }
 #pragma unroll
                         for (int half = 0; half < 2; ++half) {
                             tma_load(d + L::S + half * 8192, &maps.S, 64 * half, 64 * s, at, 0, f);
@@ -348,6 +328,30 @@ __global__ void __launch_bounds__(GRADS_THREADS, 1) delta_grads_tc_kernel(const 
                     }
                     __syncwarp();
                 }
+                if (hh > 0) continue;
+                // K and Q, once the item before has been finished.  Rows behind a sequence that ends inside the packed row are
+                // the next one's: zeros in their place (K and Q only: of d_out's they reach columns that are not used)
+                const bool tail = ch.rows < 64 && ch.t0 + ch.rows < p.T;
+                if (n_item > 0) wait(bar(G_KQ_FREE), (n_item - 1) & 1);
+                const uint32_t b = bar(tail ? G_TAIL : G_KQ), dst = base + L::KQ;
+                if (lane == 0) {
+                    mbar_expect(b, L::KQ_BYTES);
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {
+                        tma_load(dst + half * 8192, &maps.k, 64 * half, hk, tok, b0, b);
+                        tma_load(dst + 16384 + half * 8192, &maps.q, 64 * half, hk, tok, b0, b);
+                    }
+                }
+                if (tail) {
+                    wait(b, n_tail++ & 1);
+                    for (int i = lane; i < (64 - ch.rows) * 32; i += 32)
+                        *reinterpret_cast<uint4 *>(smem + L::KQ + (i >> 3 & 3) * 8192 + (ch.rows + i / 32) * 128 + (i & 7) * 16) =
+                            make_uint4(0, 0, 0, 0);
+                    fence_async_proxy();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(bar(G_KQ));
+                }
+                ++n_item;
             }
         }
     } else if (elect_one()) {
@@ -364,7 +368,7 @@ __global__ void __launch_bounds__(GRADS_THREADS, 1) delta_grads_tc_kernel(const 
         for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
             const int slot = static_cast<int>(item / p.Hk);
             if (get_chunk(p, slot).rows == 0) continue;
-            const uint32_t keys = base + L::KQ + (n_item & 1) * L::KQ_BYTES, queries = keys + 16384;
+            const uint32_t keys = base + L::KQ, queries = keys + 16384;
             for (int hh = 0; hh < group; ++hh, ++n_head) {
                 // what D and F are made of does not wait until the head before has been read; the rest does.  Both slabs of a V
                 // up to 128 stay for that; of a longer one each slab is finished in its turn.
@@ -373,13 +377,18 @@ __global__ void __launch_bounds__(GRADS_THREADS, 1) delta_grads_tc_kernel(const 
                     wait(bar(G_SLAB + (n & 1)), (n >> 1) & 1);
                     tc_fence_after();
                     product(L::DP, d + L::E, d + L::DO, true, add);                 // [e; z] d_out^T: rows of e
+                    product(L::DP, d + L::E_LO, d + L::DO, true, true);
                     product(L::F0, d + L::E, d + L::E, false, add);                 // [e; z] e^T: rows of z
+                    product(L::F0, d + L::E_LO, d + L::E, false, true);
+                    product(L::F0, d + L::E, d + L::E_LO, false, true);
                 };
                 const auto second = [&](uint32_t n, bool add) {
                     const uint32_t d = base + (n & 1) * L::SLAB;
                     product(L::DQ1, d + L::S, d + L::DO, true, add);
                     product(L::DR1, d + L::S, d + L::Z, false, add);
+                    product(L::DR1, d + L::S, d + L::Z_LO, false, true);
                     product(L::DW1, d + L::DS, d + L::E, false, add);
+                    product(L::DW1, d + L::DS, d + L::E_LO, false, true);
                     tc_commit(bar(G_SLAB_FREE + (n & 1)));
                 };
                 const auto read_before = [&] {
@@ -400,7 +409,7 @@ __global__ void __launch_bounds__(GRADS_THREADS, 1) delta_grads_tc_kernel(const 
                     tc_commit(bar(G_ACC));
                 }
                 n_slab += slabs;
-                if (hh == 0) wait(bar(G_KQ + (n_item & 1)), (n_item >> 1) & 1);
+                if (hh == 0) wait(bar(G_KQ), n_item & 1);
                 wait(bar(G_DF), n_head & 1);
                 tc_fence_after();
 #pragma unroll
@@ -422,9 +431,9 @@ __global__ void __launch_bounds__(GRADS_THREADS, 1) delta_grads_tc_kernel(const 
 }
 
 // rows of `cols` bf16 in [outer][Vp][cols] scratch, in boxes of 64 x 64
-static int scratch_map(CUtensorMap *map, const bf16 *x, const DeltaParams &p, int cols) {
-    DeltaParams q = p;                       // (column, row, slot and head, -)
-    q.T = int64_t(p.slots) * p.H;
+static int scratch_map(CUtensorMap *map, const bf16 *x, const DeltaParams &p, int cols, int planes) {
+    DeltaParams q = p;                       // (column, row, slot and head and plane, -)
+    q.T = int64_t(p.slots) * p.H * planes;
     q.batch = 1;
     const Planes pl = {x, 0, 0, int64_t(p.Vp) * cols, cols};
     return make_box_map(map, pl, q, cols, p.Vp, 64, 64, 1, true);
@@ -437,10 +446,10 @@ int delta_launch_grads_tc(const DeltaParams &p, int sm_count, cudaStream_t st) {
     if ((rc = make_map(&maps.k, p.k, p, p.Kp, p.Hk, 64, true)) != ASCAN_OK) return rc;
     if ((rc = make_map(&maps.q, p.q, p, p.Kp, p.Hk, 64, true)) != ASCAN_OK) return rc;
     if ((rc = make_map(&maps.d_out, p.d_out, p, p.Vp, p.H, 64, true)) != ASCAN_OK) return rc;
-    if ((rc = scratch_map(&maps.e, p.e, p, 64)) != ASCAN_OK) return rc;
-    if ((rc = scratch_map(&maps.z, p.z, p, 64)) != ASCAN_OK) return rc;
-    if ((rc = scratch_map(&maps.S, p.S, p, 128)) != ASCAN_OK) return rc;
-    if ((rc = scratch_map(&maps.dS, p.dS, p, 128)) != ASCAN_OK) return rc;
+    if ((rc = scratch_map(&maps.e, p.e, p, 64, 2)) != ASCAN_OK) return rc;
+    if ((rc = scratch_map(&maps.z, p.z, p, 64, 2)) != ASCAN_OK) return rc;
+    if ((rc = scratch_map(&maps.S, p.S, p, p.Kp <= 64 ? 64 : 128, 1)) != ASCAN_OK) return rc;
+    if ((rc = scratch_map(&maps.dS, p.dS, p, p.Kp <= 64 ? 64 : 128, 1)) != ASCAN_OK) return rc;
     const auto kernel = p.H == p.Hk ? delta_grads_tc_kernel<false> : delta_grads_tc_kernel<true>;
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, TcGrads::BYTES) != cudaSuccess) return ASCAN_ERR_LAUNCH;
     const int64_t items = int64_t(p.slots) * p.Hk;

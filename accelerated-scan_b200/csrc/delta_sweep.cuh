@@ -7,60 +7,51 @@
 namespace ascan {
 
 // rows of 16 columns (v0 ..) of a warp's 64 x 16 result that lies transposed in accumulators: out (any type)
-template <int NT>
 __device__ __forceinline__ void stage_transposed(uint32_t stg, unsigned char *stg_p, const float (&c)[8][4], int lane) {
-    if (NT == 1) {           // bf16, [piece][token] of 16 bytes
+    // fp32, [v / 4][token] of 16 bytes
+    float *f = reinterpret_cast<float *>(stg_p);
 #pragma unroll
-        for (int np = 0; np < 4; ++np) {
-            const int m = lane >> 3;     // matrices: (tokens 16 np, piece 0), (.., piece 1), (tokens + 8, 0), (.., 1)
-            const uint32_t a = stg + ((m & 1) * 64 + 16 * np + (m >> 1) * 8 + (lane & 7)) * 16;
-            stsm4t(a, pack2(c[2 * np][0], c[2 * np][1]), pack2(c[2 * np][2], c[2 * np][3]),
-                   pack2(c[2 * np + 1][0], c[2 * np + 1][1]), pack2(c[2 * np + 1][2], c[2 * np + 1][3]));
+    for (int n = 0; n < 8; ++n)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int v = (lane >> 2) + (j >> 1) * 8, t = 8 * n + 2 * (lane & 3) + (j & 1);
+            f[((v >> 2) * 64 + t) * 4 + (v & 3)] = c[n][j];
         }
-    } else {                 // fp32, [v / 4][token] of 16 bytes
-        float *f = reinterpret_cast<float *>(stg_p);
-#pragma unroll
-        for (int n = 0; n < 8; ++n)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int v = (lane >> 2) + (j >> 1) * 8, t = 8 * n + 2 * (lane & 3) + (j & 1);
-                f[((v >> 2) * 64 + t) * 4 + (v & 3)] = c[n][j];
-            }
-    }
 }
 
 // ... to a (token, v) array of the storage type; rows tokens, columns v0 .. of V
-template <int NT>
 __device__ __forceinline__ void flush_out(const unsigned char *stg, void *dst, int dtype, int64_t base, int64_t row_stride, int rows,
                                           int v0, int V, int lane) {
     for (int i = lane; i < 128; i += 32) {
         const int t = i >> 1, pc = i & 1, v = v0 + pc * 8;
         if (t >= rows || v >= V) continue;
         const int64_t at = base + t * row_stride + v;
-        if (NT == 1) {
-            const uint4 x = *reinterpret_cast<const uint4 *>(stg + (pc * 64 + t) * 16);
-            bf16 *o = static_cast<bf16 *>(dst) + at;
-            if (V % 8 == 0) {
-                *reinterpret_cast<uint4 *>(o) = x;
-            } else {
-                const bf16 *s = reinterpret_cast<const bf16 *>(&x);
-                for (int j = 0; j < 8 && v + j < V; ++j) o[j] = s[j];
-            }
+        const float *f = reinterpret_cast<const float *>(stg) + (2 * pc * 64 + t) * 4;
+        const float4 x = *reinterpret_cast<const float4 *>(f), y = *reinterpret_cast<const float4 *>(f + 256);
+        if (V % 8) {
+            const float e[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (v + j < V) store_from_float(dst, dtype, at + j, e[j]);
+        } else if (dtype == ASCAN_F32) {
+            float4 *o = reinterpret_cast<float4 *>(static_cast<float *>(dst) + at);
+            o[0] = x;
+            o[1] = y;
         } else {
-            const float *f = reinterpret_cast<const float *>(stg);
-            for (int j = 0; j < 8 && v + j < V; ++j) store_from_float(dst, dtype, at + j, f[((2 * pc + (j >> 2)) * 64 + t) * 4 + (j & 3)]);
+            alignas(16) const __half2 h[4] = {__floats2half2_rn(x.x, x.y), __floats2half2_rn(x.z, x.w), __floats2half2_rn(y.x, y.y), __floats2half2_rn(y.z, y.w)};
+            *reinterpret_cast<uint4 *>(static_cast<__half *>(dst) + at) = *reinterpret_cast<const uint4 *>(h);
         }
     }
 }
 
 // the warp's 16 x KP accumulators (of the state, or KP = 64 tokens of e or z) to bf16 planes [plane][Vp][KP], through the
 // staging area
-template <int KP, int NT>
+template <int KP>
 __device__ __forceinline__ void save_state(uint32_t stg, const unsigned char *stg_p, const float (&s)[KP / 8][4], bf16 *dst, int v0,
                                            int Vp, int lane) {
     constexpr int NCH = KP / 8;
 #pragma unroll
-    for (int pl = 0; pl < NT; ++pl) {
+    for (int pl = 0; pl < 2; ++pl) {
         __syncwarp();
 #pragma unroll
         for (int kk = 0; kk < KP / 16; ++kk) {
