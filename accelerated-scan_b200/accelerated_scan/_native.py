@@ -514,6 +514,8 @@ def _sink(device):
     raises."""
     sink = _sinks.get(device.index)
     if sink is None:
+        if torch.cuda.is_current_stream_capturing():     # nothing may be allocated now: these launches have no word to set
+            return 0
         word = torch.zeros(4, dtype=torch.int32).pin_memory()
         sink = _sinks[device.index] = (word, word.numpy(), word.data_ptr())
     if sink[1][0]:

@@ -461,6 +461,7 @@ __global__ void __launch_bounds__(STEP_THREADS, 1) delta_step_ring_kernel(const 
         }
     }
     if (tid == 0) tma_store_done();
+    drain(&dead_flag);
 }
 
 }  // namespace ascan

@@ -53,11 +53,12 @@ __device__ __forceinline__ void back_load(const DeltaParams &p, uint32_t base, c
 }
 
 template <int KP>
-__global__ void __launch_bounds__(256, 1) delta_back_sweep_kernel(DeltaParams p) {
+__global__ void __launch_bounds__(256, 1) delta_back_sweep_kernel(DeltaParams p, int warps) {
     extern __shared__ __align__(128) unsigned char smem[];
     typedef BackLayout<KP> L;
     constexpr int NCH = KP / 8, KT = KP / 8;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, threads = blockDim.x, warps = threads >> 5;
+    constexpr int threads = SWEEP_THREADS;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int g = lane >> 2, t2 = 2 * (lane & 3);
     const int cta_cols = 16 * warps, slices = (p.Vp + cta_cols - 1) / cta_cols;
     const int slice = blockIdx.x % slices;
@@ -75,7 +76,7 @@ __global__ void __launch_bounds__(256, 1) delta_back_sweep_kernel(DeltaParams p)
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const int k = 8 * n + t2 + (j & 1), v = v0 + g + (j >> 1) * 8;
-            s[n][j] = p.d_s1 && k < p.K && v < p.V ? p.d_s1[state_at + int64_t(k) * p.V + v] : 0.f;
+            s[n][j] = p.d_s1 && warp < warps && k < p.K && v < p.V ? p.d_s1[state_at + int64_t(k) * p.V + v] : 0.f;
         }
 
     if (sq.chunks > 0) {
@@ -86,7 +87,11 @@ __global__ void __launch_bounds__(256, 1) delta_back_sweep_kernel(DeltaParams p)
         if (c > 0) back_load<KP>(p, base + (turn ^ 1) * stage_bytes, sq, c - 1, h, hk, v0_cta, warps, tid, threads);
         cp_commit();
         cp_wait<1>();
-        __syncthreads();
+        sweep_sync();
+        if (warp >= warps) {           // loads only
+            sweep_sync();
+            continue;
+        }
         const uint32_t st = base + turn * stage_bytes;
         const float *sc = reinterpret_cast<const float *>(smem + turn * stage_bytes + L::SC);
         const int64_t at = int64_t(sq.slot0 + c) * p.H + h;
@@ -226,10 +231,10 @@ __global__ void __launch_bounds__(256, 1) delta_back_sweep_kernel(DeltaParams p)
                 mma(s[2 * np + 1], as[0], b[2], b[3]);
             }
         }
-        __syncthreads();
+        sweep_sync();
     }
     cp_wait<0>();
-    if (p.d_s0) {
+    if (p.d_s0 && warp < warps) {
 #pragma unroll
         for (int n = 0; n < KT; ++n)
 #pragma unroll
@@ -248,7 +253,7 @@ static int launch_back_sweep(const DeltaParams &p, int sm_count, cudaStream_t st
     if (grid > 0x7fffffff) return ASCAN_ERR_UNSUPPORTED;
     if (cudaFuncSetAttribute(delta_back_sweep_kernel<KP>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)) != cudaSuccess)
         return ASCAN_ERR_LAUNCH;
-    delta_back_sweep_kernel<KP><<<unsigned(grid), 32 * warps, smem, st>>>(p);
+    delta_back_sweep_kernel<KP><<<unsigned(grid), SWEEP_THREADS, smem, st>>>(p, warps);
     return cudaGetLastError() == cudaSuccess ? ASCAN_OK : ASCAN_ERR_LAUNCH;
 }
 

@@ -324,11 +324,12 @@ __device__ __forceinline__ void sweep_load(const DeltaParams &p, uint32_t base, 
 }
 
 template <int KP, bool SAVE>
-__global__ void __launch_bounds__(256, 1) delta_sweep_kernel(DeltaParams p) {
+__global__ void __launch_bounds__(256, 1) delta_sweep_kernel(DeltaParams p, int warps) {
     extern __shared__ __align__(128) unsigned char smem[];
     typedef SweepLayout<KP> L;
     constexpr int NCH = KP / 8, KT = KP / 8;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, threads = blockDim.x, warps = threads >> 5;
+    constexpr int threads = SWEEP_THREADS;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int g = lane >> 2, t2 = 2 * (lane & 3);
     const int cta_cols = 16 * warps, slices = (p.Vp + cta_cols - 1) / cta_cols;
     const int slice = blockIdx.x % slices;
@@ -346,7 +347,7 @@ __global__ void __launch_bounds__(256, 1) delta_sweep_kernel(DeltaParams p) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const int k = 8 * n + t2 + (j & 1), v = v0 + g + (j >> 1) * 8;
-            s[n][j] = p.s0 && k < p.K && v < p.V ? p.s0[state_at + int64_t(k) * p.V + v] : 0.f;
+            s[n][j] = p.s0 && warp < warps && k < p.K && v < p.V ? p.s0[state_at + int64_t(k) * p.V + v] : 0.f;
         }
 
     if (sq.chunks > 0) {
@@ -357,7 +358,11 @@ __global__ void __launch_bounds__(256, 1) delta_sweep_kernel(DeltaParams p) {
         if (c + 1 < sq.chunks) sweep_load<KP>(p, base + ((c + 1) & 1) * stage_bytes, sq, c + 1, h, hk, v0_cta, warps, tid, threads);
         cp_commit();
         cp_wait<1>();
-        __syncthreads();
+        sweep_sync();
+        if (warp >= warps) {           // loads only
+            sweep_sync();
+            continue;
+        }
         const uint32_t st = base + (c & 1) * stage_bytes;
         const float *sc = reinterpret_cast<const float *>(smem + (c & 1) * stage_bytes + L::SC);
         const int64_t at = int64_t(sq.slot0 + c) * p.H + h;
@@ -496,7 +501,7 @@ __global__ void __launch_bounds__(256, 1) delta_sweep_kernel(DeltaParams p) {
         __syncwarp();
         const int64_t t0 = sq.t0 + int64_t(c) * 64;
         flush_out(stg_p, p.out, p.dtype, ((sq.b * p.T + t0) * p.H + h) * int64_t(p.V), int64_t(p.H) * p.V, rows, v0, p.V, lane);
-        __syncthreads();
+        sweep_sync();
     }
     cp_wait<0>();
 #pragma unroll
@@ -504,12 +509,12 @@ __global__ void __launch_bounds__(256, 1) delta_sweep_kernel(DeltaParams p) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const int k = 8 * n + t2 + (j & 1), v = v0 + g + (j >> 1) * 8;
-            if (k < p.K && v < p.V) p.s1[state_at + int64_t(k) * p.V + v] = s[n][j];
+            if (warp < warps && k < p.K && v < p.V) p.s1[state_at + int64_t(k) * p.V + v] = s[n][j];
         }
     if (p.packed && (n_seq == 0 || n_seq == p.n_seqs - 1)) {      // tokens of no sequence: zeros
         const int64_t front = n_seq == 0 ? sq.t0 : 0, back = n_seq == p.n_seqs - 1 ? sq.t0 + sq.len : p.T;
         const int64_t rows = front + (p.T - back);
-        for (int64_t i = warp * 32 + lane; i < rows * cta_cols; i += threads) {
+        for (int64_t i = tid; i < rows * cta_cols; i += threads) {
             const int64_t r = i / cta_cols;
             const int v = v0_cta + static_cast<int>(i % cta_cols);
             if (v < p.V) store_from_float(p.out, p.dtype, ((r < front ? r : back + (r - front)) * p.H + h) * p.V + v, 0.f);
@@ -525,7 +530,7 @@ static int launch_sweep(const DeltaParams &p, int sm_count, cudaStream_t st) {
     if (grid > 0x7fffffff) return ASCAN_ERR_UNSUPPORTED;
     if (cudaFuncSetAttribute(delta_sweep_kernel<KP, SAVE>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)) != cudaSuccess)
         return ASCAN_ERR_LAUNCH;
-    delta_sweep_kernel<KP, SAVE><<<unsigned(grid), 32 * warps, smem, st>>>(p);
+    delta_sweep_kernel<KP, SAVE><<<unsigned(grid), SWEEP_THREADS, smem, st>>>(p, warps);
     return cudaGetLastError() == cudaSuccess ? ASCAN_OK : ASCAN_ERR_LAUNCH;
 }
 

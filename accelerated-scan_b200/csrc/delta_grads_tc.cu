@@ -427,6 +427,7 @@ __global__ void __launch_bounds__(GRADS_THREADS, 1) delta_grads_tc_kernel(const 
     __syncwarp();
     tc_fence_before();
     __syncthreads();
+    drain(dead);
     if (warp == GRADS_WARPS + 1) tmem_dealloc(tmem, 512);
 }
 

@@ -75,8 +75,12 @@ __device__ __forceinline__ void save_state(uint32_t stg, const unsigned char *st
     __syncwarp();
 }
 
-// Warps of a CTA: eight share one copy of the chunk's tiles where shared memory holds their own ones as well; fewer
-// while that would leave SMs without a CTA.
+// Warps of a CTA that carry columns: eight share one copy of the chunk's tiles where shared memory holds their own ones as
+// well; fewer while that would leave SMs without a CTA.  All eight load: with one warp for its own tiles, 100 KB a chunk
+// and 200 copies a thread, loading took half of the time (1000 fp32 tokens, 8 heads of 128 x 64: 247 us a sweep, now 132).
+constexpr int SWEEP_THREADS = 256;
+__device__ __forceinline__ void sweep_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
+
 static inline int sweep_warps(const DeltaParams &p, int sm_count, size_t (*bytes)(int)) {
     const int64_t slices = (p.Vp + 15) / 16, chains = int64_t(p.n_seqs) * p.H;
     int w = 8;

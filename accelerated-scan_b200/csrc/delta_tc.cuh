@@ -22,7 +22,8 @@ __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
 }
 
 // Every wait ends: after WAIT_TRIES the CTA is given up (`dead`, in shared memory), from then on no wait of the CTA
-// waits, the kernel runs to its end on whatever is in its buffers, and the host reads the status word.
+// waits, the kernel runs to its end on whatever is in its buffers, leaves its copies time to land, and the host reads
+// the status word.
 constexpr uint32_t WAIT_TRIES = 1u << 21;
 struct Waiter {
     volatile int *dead;
@@ -39,6 +40,12 @@ struct Waiter {
         }
     }
 };
+
+// Before a CTA ends: one that was given up may have copies in flight, which end by themselves within microseconds.
+__device__ __forceinline__ void drain(volatile const int *dead) {
+    if (*dead)
+        for (int i = 0; i < 1000; ++i) __nanosleep(1000);
+}
 
 template <int ID, int THREADS>
 __device__ __forceinline__ void group_sync() {
@@ -107,16 +114,6 @@ __device__ __forceinline__ void tmem_ld16(uint32_t (&r)[16], uint32_t a) {
 __device__ __forceinline__ void tmem_ld8(uint32_t (&r)[8], uint32_t a) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];" : ASCAN_R8(r, 0) : "r"(a));
 }
-__device__ __forceinline__ void tmem_st32(uint32_t a, const uint32_t (&r)[32]) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,"
-                 "%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};"
-                 :: "r"(a), ASCAN_I8(r, 0), ASCAN_I8(r, 8), ASCAN_I8(r, 16), ASCAN_I8(r, 24) : "memory");
-}
-__device__ __forceinline__ void tmem_st16(uint32_t a, const uint32_t (&r)[16]) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
-                 :: "r"(a), ASCAN_I8(r, 0), ASCAN_I8(r, 8) : "memory");
-}
-
 __device__ __forceinline__ void tmem_st8(uint32_t a, const uint32_t (&r)[8]) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" :: "r"(a), ASCAN_I8(r, 0) : "memory");
 }

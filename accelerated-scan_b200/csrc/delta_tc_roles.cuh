@@ -156,6 +156,7 @@ __device__ __forceinline__ void tc_end(const TcBlock &k) {
     __syncwarp();
     tc_fence_before();
     __syncthreads();
+    drain(k.wait.dead);
     if (threadIdx.x >> 5 == 16) tmem_dealloc(k.tmem, 512);
 }
 

@@ -349,6 +349,7 @@ __global__ void __launch_bounds__(E == 8 ? 256 : 512, E == 8 ? 3 : 1) norm_forwa
             if (live) store_row<T, ALIGNED>(p.normed, row * p.D, gt, G, p.D, r);
         }
     }
+    if (RING) drain(&gave_up);
 }
 
 // WIDE: rows whose threads have only 64 registers each.  The weights are read where they are used (from the L1 cache) and
@@ -475,6 +476,7 @@ __global__ void __launch_bounds__(WIDE ? NORM_THREADS : NORM_NARROW) norm_backwa
         }
         if (live) store_row<T, ALIGNED>(p.d_x, row * p.D, gt, G, p.D, dh);
     }
+    if (RING) drain(&gave_up);
     if (!p.partial) return;
     if (RING && slots > 1) __syncthreads();               // the sums take the ring's place
     float *to = p.partial + int64_t(blockIdx.x) * 3 * p.D;

@@ -572,3 +572,75 @@ def test_bad_arguments_of_the_c_entries():
         setattr(t, name, 256)
     assert _native.lib.ascan_delta_step(ctypes.byref(t), fake, fake, 1, 256, None, 0, None) == 1       # pool of one for two rows
     assert _native.lib.ascan_delta_step(ctypes.byref(t), fake, fake, 2, 255, None, 0, None) == 1       # states overlap
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("shape", [(8, 650, 4, 8, 72, 200), (4, 700, 4, 4, 128, 64), (3, 600, 6, 18, 64, 128)])
+def test_more_chunks_than_the_gpu_holds(cuda_device, shape, dtype):
+    """Chunks times key heads beyond the number of SMs, with one, two and four slabs of V and one to three value heads."""
+    args = inputs(sum(shape), *shape, dtype, cuda_device)
+    leaves = [t.requires_grad_(True) for t in args]
+    want, want_s = reference(*args)
+    d_out, d_s = torch.randn_like(want).to(dtype), torch.randn_like(want_s).float()
+    out, s = delta.scan(*args)
+    assert off(out, want) <= TOL[dtype] and off(s, want_s) <= CARRIED
+    want_g = torch.autograd.grad([want, want_s], leaves, [d_out.double(), d_s.double()])
+    got_g = torch.autograd.grad([out, s], leaves, [d_out, d_s])
+    for i, (a, b) in enumerate(zip(got_g, want_g)):
+        assert off(a, b) <= (CARRIED if i == 5 else TOL[dtype]) * (2 if i == 3 else 1), i
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_many_short_sequences_beside_tokens_that_are_not_finite(cuda_device, dtype):
+    """Every chunk ends inside the row; what stands in no sequence is infinite or NaN."""
+    lengths = [37, 1, 64, 5, 90, 66, 0, 23] * 8
+    T, n, front = sum(lengths) + 11, len(lengths), 6
+    args = inputs(T, 1, T, 4, 8, 128, 136, dtype, cuda_device, n=n)
+    starts = (torch.tensor([0] + lengths).cumsum(0) + front).to(torch.int32).to(cuda_device)
+    inside = slice(front, front + sum(lengths))
+    clean = [t[:, inside].clone().requires_grad_(True) for t in args[:5]] + [args[5].clone().requires_grad_(True)]
+    want, want_s = reference(*clean, lengths=lengths)
+    for i, t in enumerate(args[:5]):
+        t[:, :front] = float("nan") if i % 2 else float("inf")
+        t[:, front + sum(lengths):] = float("inf") if i % 2 else float("nan")
+    leaves = [t.requires_grad_(True) for t in args]
+    out, s = delta.scan(*args, seq_starts=starts)
+    assert off(out[:, inside], want) <= TOL[dtype] and off(s, want_s) <= CARRIED
+    d_out, d_s = torch.randn_like(out), torch.randn_like(s)
+    want_g = torch.autograd.grad([want, want_s], clean, [d_out[:, inside].double(), d_s.double()])
+    d_out[:, :front] = d_out[:, front + sum(lengths):] = float("nan")
+    got_g = torch.autograd.grad([out, s], leaves, [d_out, d_s])
+    for i, (a, b) in enumerate(zip(got_g, want_g)):
+        tol = (CARRIED if i == 5 else TOL[dtype]) * (2 if i == 3 else 1)
+        assert off(a[:, inside] if i < 5 else a, b) <= tol, i
+        if i < 5:
+            assert (a[:, :front] == 0).all() and (a[:, front + sum(lengths):] == 0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_boundaries_outside_of_the_row_are_cut_off(cuda_device, dtype):
+    args = inputs(9, 1, 150, 1, 2, 64, 64, dtype, cuda_device, n=3)
+    leaves = [t.requires_grad_(True) for t in args]
+    results = []
+    for bounds in ([-5, 30, 150, 9000], [0, 30, 150, 150]):
+        starts = torch.tensor(bounds, device=cuda_device)
+        out, s = delta.scan(*args, seq_starts=starts)
+        results.append((out, s, *torch.autograd.grad([out, s], leaves, [torch.ones_like(out), torch.ones_like(s)])))
+    for a, b in zip(*results):
+        assert torch.equal(a, b)
+
+
+def test_an_expired_wait_is_reported_once(monkeypatch):
+    """The word that a kernel sets when it gives up is read, and cleared, by the next call on its device."""
+    from accelerated_scan import _native
+    word = torch.zeros(4, dtype=torch.int32)
+    monkeypatch.setattr(_native, "_sinks", {0: (word, word.numpy(), word.data_ptr())})
+    device = torch.device("cuda", 0)
+    assert _native._sink(device) == word.data_ptr()
+    word[0] = 1
+    with pytest.raises(RuntimeError, match="wait expired"):
+        _native._sink(device)
+    assert _native._sink(device) == word.data_ptr()
