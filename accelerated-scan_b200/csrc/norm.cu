@@ -22,7 +22,7 @@ struct NormParams {
     void *hidden, *normed;
     const void *d_hidden, *d_normed;
     void *d_x, *d_residual, *d_gate;
-    float *partial;                                 // [grid][3][D]: post, scale, pre
+    float *partial;                                 // [grid][2][D]: post and scale (below), pre
     int32_t stages;                                 // of the copies' ring; 0: plain loads
     int *status;                                    // nullable: set when a wait for a copy expired
 };
@@ -223,16 +223,11 @@ struct RowSum {
     }
     template <int N>
     __device__ __forceinline__ void operator()(float (&v)[N]) {
-        if (lanes == 32) {
 #pragma unroll
-            for (int d = 16; d; d /= 2)
-#pragma unroll
-                for (int j = 0; j < N; ++j) v[j] += __shfl_xor_sync(~0u, v[j], d);
-        } else {
-            for (int d = lanes / 2; d; d /= 2)
+        for (int d = 16; d; d /= 2)
+            if (d < lanes)
 #pragma unroll
                 for (int j = 0; j < N; ++j) v[j] += __shfl_xor_sync(~0u, v[j], d);
-        }
         if (warps == 0) return;
         float *r = red + turn * 2 * 32;
         turn ^= 1;
@@ -352,12 +347,14 @@ __global__ void __launch_bounds__(E == 8 ? 256 : 512, E == 8 ? 3 : 1) norm_forwa
     if (RING) drain(&gave_up);
 }
 
-// WIDE: rows whose threads have only 64 registers each.  The weights are read where they are used (from the L1 cache) and
+// With x' the normed x, z the gate's value and dh the gradient of h: sum over rows of dh z x' is the gradient of post_weight but
+// for the factor scale, and that of scale but for the factor post_weight, so one sum serves both, and one product of the two
+// weights the rest.  WIDE: rows whose threads have only 64 registers each.  The weights are read where they are used (from the L1 cache) and
 // their gradients are summed in shared memory, by the thread that owns the element.
 template <class T, bool ALIGNED, bool WIDE, bool RING>
 __global__ void __launch_bounds__(WIDE ? NORM_THREADS : NORM_NARROW) norm_backward_kernel(const __grid_constant__ NormParams p) {
     extern __shared__ __align__(128) unsigned char dynamic[];
-    float *sums = reinterpret_cast<float *>(dynamic);     // [slots][3][D] when rows share a CTA; WIDE: [3][EPT][threads]
+    float *sums = reinterpret_cast<float *>(dynamic);     // [slots][2][D] when rows share a CTA; WIDE: [2][EPT][threads]
     __shared__ __align__(16) float red[2 * 2 * 32];
     __shared__ uint64_t bar[8];
     __shared__ int gave_up;
@@ -365,22 +362,27 @@ __global__ void __launch_bounds__(WIDE ? NORM_THREADS : NORM_NARROW) norm_backwa
     const int G = p.groups, slots = blockDim.x / G, gt = threadIdx.x % G, slot = threadIdx.x / G;
     const float inv_d = 1.f / float(p.D);
     RowSum row_sum(red, G);
-    float pw[EPT], sc[EPT], qw[EPT], d_w[WIDE ? 1 : 3][EPT] = {};
+    float w[EPT], qw[EPT], d_w[WIDE ? 1 : 2][EPT] = {};         // w: scale and post_weight in one
+    const auto load_w = [&] {
+        load_weight<T, ALIGNED>(p.post_w, p.w_dtype, gt, G, p.D, 1.f, w);
+        load_weight<T, ALIGNED>(p.scale, p.w_dtype, gt, G, p.D, p.scale_value, qw);
+#pragma unroll
+        for (int i = 0; i < EPT; ++i) w[i] *= qw[i];
+    };
     if (!WIDE) {
-        load_weight<T, ALIGNED>(p.post_w, p.w_dtype, gt, G, p.D, 1.f, pw);
-        load_weight<T, ALIGNED>(p.scale, p.w_dtype, gt, G, p.D, p.scale_value, sc);
+        load_w();
         load_weight<T, ALIGNED>(p.pre_w, p.w_dtype, gt, G, p.D, 1.f, qw);
     } else if (p.partial) {
-        for (int i = 0; i < 3 * EPT; ++i) sums[i * blockDim.x + threadIdx.x] = 0.f;
+        for (int i = 0; i < 2 * EPT; ++i) sums[i * blockDim.x + threadIdx.x] = 0.f;
     }
     // the ring lies behind the sums where these are kept from the start, and in their place else
-    RowRing<T, 5> ring(p, dynamic + (WIDE && p.partial ? 3 * EPT * blockDim.x * 4 : 0), bar, &gave_up, slots);
+    RowRing<T, 5> ring(p, dynamic + (WIDE && p.partial ? 2 * EPT * blockDim.x * 4 : 0), bar, &gave_up, slots);
     if (RING) {
         ring.src[0] = p.x; ring.src[1] = p.residual; ring.src[2] = p.gate; ring.src[3] = p.d_hidden; ring.src[4] = p.d_normed;
         ring.stride[0] = p.x_s; ring.stride[1] = p.r_s; ring.stride[2] = p.g_s; ring.stride[3] = p.dh_s; ring.stride[4] = p.dy_s;
         ring.init();
     }
-    const auto add = [&](int which, int i, float x) {     // post, scale, pre
+    const auto add = [&](int which, int i, float x) {     // post and scale, pre
         if (!WIDE) d_w[WIDE ? 0 : which][i] += x;
         else if (p.partial) sums[(which * EPT + i) * blockDim.x + threadIdx.x] += x;
     };
@@ -413,10 +415,6 @@ __global__ void __launch_bounds__(WIDE ? NORM_THREADS : NORM_NARROW) norm_backwa
             row_sum(s);
             rx = rsqrtf(s[0] * inv_d + p.eps);
         }
-        if (WIDE) {
-            load_weight<T, ALIGNED>(p.post_w, p.w_dtype, gt, G, p.D, 1.f, pw);
-            load_weight<T, ALIGNED>(p.scale, p.w_dtype, gt, G, p.D, p.scale_value, sc);
-        }
         float slope[EPT];
         if (p.gate) {
             open_gates<true>(z, slope, p.act);                            // from here on the gate's value
@@ -428,11 +426,11 @@ __global__ void __launch_bounds__(WIDE ? NORM_THREADS : NORM_NARROW) norm_backwa
             }
         }
 #pragma unroll
-        for (int i = 0; i < EPT; ++i) {
-            x[i] *= rx;                                                   // ... and the normed x
-            h[i] += sc[i] * (z[i] * (x[i] * pw[i]));
-        }
+        for (int i = 0; i < EPT; ++i) x[i] *= rx;                         // ... and the normed x
+        if (WIDE) load_w();
         if (p.d_normed) {
+#pragma unroll
+            for (int i = 0; i < EPT; ++i) h[i] += w[i] * (z[i] * x[i]);
             if (WIDE) load_weight<T, ALIGNED>(p.pre_w, p.w_dtype, gt, G, p.D, 1.f, qw);
             float s[2] = {};
 #pragma unroll
@@ -444,31 +442,24 @@ __global__ void __launch_bounds__(WIDE ? NORM_THREADS : NORM_NARROW) norm_backwa
             const float rh = rsqrtf(s[0] * inv_d + p.eps), c = s[1] * rh * rh * inv_d;
 #pragma unroll
             for (int i = 0; i < EPT; ++i) {
-                add(2, i, dy[i] * (h[i] * rh));
+                add(1, i, dy[i] * (h[i] * rh));
                 dh[i] += rh * (dy[i] * qw[i] - h[i] * c);
             }
         }
         if (p.d_residual && live) store_row<T, ALIGNED>(p.d_residual, row * p.D, gt, G, p.D, dh);
-        if (WIDE) {
-            load_weight<T, ALIGNED>(p.post_w, p.w_dtype, gt, G, p.D, 1.f, pw);
-            load_weight<T, ALIGNED>(p.scale, p.w_dtype, gt, G, p.D, p.scale_value, sc);
-        }
+        if (WIDE && p.d_normed) load_w();
+        float s[1] = {};
 #pragma unroll
         for (int i = 0; i < EPT; ++i) {
-            const float n = x[i] * pw[i];
-            add(1, i, dh[i] * (z[i] * n));
-            slope[i] *= dh[i] * sc[i] * n;                                // gradient of the gate
-            dh[i] *= sc[i] * z[i];                                        // gradient of n
+            slope[i] *= dh[i] * (x[i] * w[i]);                            // gradient of the gate
+            dh[i] *= z[i];
+            const float a = dh[i] * x[i];
+            add(0, i, a);
+            dh[i] *= w[i];                                                // gradient of the normed x
+            s[0] += a * w[i];
         }
         if (p.d_gate && live) store_row<T, ALIGNED>(p.d_gate, row * p.D, gt, G, p.D, slope);
         if (p.post_w) {
-            float s[1] = {};
-#pragma unroll
-            for (int i = 0; i < EPT; ++i) {
-                add(0, i, dh[i] * x[i]);
-                dh[i] *= pw[i];
-                s[0] += dh[i] * x[i];
-            }
             row_sum(s);
             const float c = s[0] * inv_d;
 #pragma unroll
@@ -479,45 +470,48 @@ __global__ void __launch_bounds__(WIDE ? NORM_THREADS : NORM_NARROW) norm_backwa
     if (RING) drain(&gave_up);
     if (!p.partial) return;
     if (RING && slots > 1) __syncthreads();               // the sums take the ring's place
-    float *to = p.partial + int64_t(blockIdx.x) * 3 * p.D;
+    float *to = p.partial + int64_t(blockIdx.x) * 2 * p.D;
 #pragma unroll
     for (int i = 0; i < EPT; ++i) {
         const int e = element<T, ALIGNED>(i, gt, G);
         if (e >= p.D) continue;
 #pragma unroll
-        for (int w = 0; w < 3; ++w) {
-            const float v = WIDE ? sums[(w * EPT + i) * blockDim.x + threadIdx.x] : d_w[WIDE ? 0 : w][i];
-            if (slots > 1) sums[(slot * 3 + w) * p.D + e] = v;
-            else to[w * p.D + e] = v;
+        for (int j = 0; j < 2; ++j) {
+            const float v = WIDE ? sums[(j * EPT + i) * blockDim.x + threadIdx.x] : d_w[WIDE ? 0 : j][i];
+            if (slots > 1) sums[(slot * 2 + j) * p.D + e] = v;
+            else to[j * p.D + e] = v;
         }
     }
     if (slots > 1) {                                      // never WIDE
         __syncthreads();
-        for (int i = threadIdx.x; i < 3 * p.D; i += blockDim.x) {
+        for (int i = threadIdx.x; i < 2 * p.D; i += blockDim.x) {
             float s = 0.f;
-            for (int k = 0; k < slots; ++k) s += sums[k * 3 * p.D + i];
+            for (int k = 0; k < slots; ++k) s += sums[k * 2 * p.D + i];
             to[i] = s;
         }
     }
 }
 
 // Weights' gradients from the CTAs' sums: 32 columns by 32 threads a CTA, CTAs' sums added in a fixed order.
-__global__ void __launch_bounds__(1024) norm_weights_kernel(const float *partial, int parts, int D, int w_dtype, void *d_post, void *d_scale,
+__global__ void __launch_bounds__(1024) norm_weights_kernel(const __grid_constant__ NormParams p, int parts, void *d_post, void *d_scale,
                                                             void *d_pre) {
     __shared__ float s[32][33];
     const int cx = threadIdx.x & 31, ry = threadIdx.x >> 5, col = blockIdx.x * 32 + cx, which = blockIdx.y;
-    void *dst = which == 0 ? d_post : which == 1 ? d_scale : d_pre;
-    if (!dst) return;
+    if (which == 0 ? !d_post && !d_scale : !d_pre) return;
     float a = 0.f;
-    if (col < D)
-        for (int r = ry; r < parts; r += 32) a += partial[(int64_t(r) * 3 + which) * D + col];
+    if (col < p.D)
+        for (int r = ry; r < parts; r += 32) a += p.partial[(int64_t(r) * 2 + which) * p.D + col];
     s[ry][cx] = a;
     __syncthreads();
-    if (ry == 0 && col < D) {
+    if (ry == 0 && col < p.D) {
         float t = 0.f;
 #pragma unroll
         for (int r = 0; r < 32; ++r) t += s[r][cx];
-        store_from_float(dst, w_dtype, col, t);
+        if (which == 1) store_from_float(d_pre, p.w_dtype, col, t);
+        else {
+            if (d_post) store_from_float(d_post, p.w_dtype, col, t * (p.scale ? load_as_float(p.scale, p.w_dtype, col) : p.scale_value));
+            if (d_scale) store_from_float(d_scale, p.w_dtype, col, t * (p.post_w ? load_as_float(p.post_w, p.w_dtype, col) : 1.f));
+        }
     }
 }
 
@@ -581,7 +575,7 @@ template <class T, bool ALIGNED, bool WIDE>
 static int launch_back(NormParams p, int grid, int threads, cudaStream_t st) {
     const int slots = threads / p.groups;
     size_t sums = 0;
-    if (p.partial) sums = WIDE ? size_t(3) * 8 * threads * 4 : slots > 1 ? size_t(slots) * 3 * p.D * 4 : 0;   // at most 96 KB
+    if (p.partial) sums = WIDE ? size_t(2) * 8 * threads * 4 : slots > 1 ? size_t(slots) * 2 * p.D * 4 : 0;   // at most 64 KB
     p.stages = ALIGNED ? ring_stages(p, 5, slots, grid, false, sizeof(T), WIDE ? sums : 0) : 0;
     const size_t ring = size_t(p.stages) * 5 * slots * p.D * sizeof(T);
     const size_t smem = WIDE ? sums + ring : sums > ring ? sums : ring;
@@ -677,7 +671,7 @@ size_t ascan_norm_backward_bytes(const ascan_norm *a) {
         sms = 148;          // no device to ask: size for a full B200
     }
     norm_shape(p.D, 8, &p.groups, &threads);
-    return size_t(norm_grid(p.rows, p.groups, threads, sms, false)) * 3 * p.D * 4;
+    return size_t(norm_grid(p.rows, p.groups, threads, sms, false)) * 2 * p.D * 4;
 }
 
 int ascan_norm_backward(const ascan_norm *a, const void *d_hidden, int64_t d_hidden_stride, const void *d_normed, int64_t d_normed_stride,
@@ -708,8 +702,7 @@ int ascan_norm_backward(const ascan_norm *a, const void *d_hidden, int64_t d_hid
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (p.rows > 0 && (rc = launch_norm_by_type(p, a->dtype, grid, threads, aligned, true, st)) != ASCAN_OK) return rc;
     if (weights) {         // without rows: zeros
-        norm_weights_kernel<<<dim3((p.D + 31) / 32, 3), 1024, 0, st>>>(p.partial, p.rows > 0 ? grid : 0, p.D, p.w_dtype, d_post_weight,
-                                                                       d_scale, d_pre_weight);
+        norm_weights_kernel<<<dim3((p.D + 31) / 32, 2), 1024, 0, st>>>(p, p.rows > 0 ? grid : 0, d_post_weight, d_scale, d_pre_weight);
         if (cudaGetLastError() != cudaSuccess) return ASCAN_ERR_LAUNCH;
     }
     return ASCAN_OK;
