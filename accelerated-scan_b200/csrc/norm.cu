@@ -8,6 +8,10 @@
 // rounded h.  A thread holds eight elements (sixteen in the forward of long rows), 16 bytes at a time;
 // G threads share a row, and a CTA keeps the weights, and in the backward the weights' gradients, in registers over all
 // its rows.  Sums of the weights' gradients over CTAs are a second launch, in a fixed order.
+//
+// Measured, bf16: 32768 rows of 4096 with all parts, forward, 276 us (1.34 GB, 4.9 TB/s; 6.55 are a plain copy's); 262144
+// heads of 128 with a gate, forward 52 us and backward 85 us (201 and 335 MB, 3.9 TB/s).  What is missing is issue slots:
+// 2.3 - 2.7 instructions a clock, of which conversions, gates and the rows' reductions are most.
 #include <atomic>
 
 #include "delta_tc.cuh"
@@ -30,6 +34,7 @@ struct NormParams {
 constexpr int NORM_THREADS = 1024, NORM_MAX_D = 8 * NORM_THREADS;
 constexpr int NORM_NARROW = 512;                    // threads up to which the backward keeps all it needs in registers
 
+enum : int { LEAN, MIDDLE, WIDE_ROWS };
 enum : int { ACT_NONE = 0, ACT_SIGMOID = 1, ACT_SILU = 2 };
 
 template <class T> struct Elem;
@@ -124,7 +129,8 @@ __device__ __forceinline__ void store_row(void *dst, int64_t at, int gt, int G, 
 
 // Rows by bulk copies: a ring of `stages` buffers, each the rows that the CTA works on at once (`slots`) of every input, so
 // that the next rows are under way while these are reduced: with plain loads a CTA asks for nothing between its first
-// barrier and its last store.  One thread issues; rows that lie dense are one copy an input.
+// barrier and its last store.  One thread issues; rows that lie dense are one copy an input.  32768 rows of 4096, bf16: 508 us
+// with plain loads, 278 so (lighter gates and sixteen elements a thread are in it too).
 template <class T, int INPUTS>
 struct RowRing {
     const NormParams &p;
@@ -351,18 +357,19 @@ __global__ void __launch_bounds__(E == 8 ? 256 : 512, E == 8 ? 3 : 1) norm_forwa
 // for the factor scale, and that of scale but for the factor post_weight, so one sum serves both, and one product of the two
 // weights the rest.  WIDE: rows whose threads have only 64 registers each.  The weights are read where they are used (from the L1 cache) and
 // their gradients are summed in shared memory, by the thread that owns the element.
-template <class T, bool ALIGNED, bool WIDE, bool RING>
-__global__ void __launch_bounds__(WIDE ? NORM_THREADS : NORM_NARROW) norm_backward_kernel(const __grid_constant__ NormParams p) {
+template <class T, bool ALIGNED, int FORM, bool RING>
+__global__ void __launch_bounds__(FORM == LEAN ? 256 : FORM == WIDE_ROWS ? NORM_THREADS : NORM_NARROW, FORM == LEAN ? 3 : 1) norm_backward_kernel(const __grid_constant__ NormParams p) {
     extern __shared__ __align__(128) unsigned char dynamic[];
     float *sums = reinterpret_cast<float *>(dynamic);     // [slots][2][D] when rows share a CTA; WIDE: [2][EPT][threads]
     __shared__ __align__(16) float red[2 * 2 * 32];
     __shared__ uint64_t bar[8];
     __shared__ int gave_up;
     constexpr int EPT = 8;
+    constexpr bool WIDE = FORM == WIDE_ROWS, PRE = FORM != LEAN;
     const int G = p.groups, slots = blockDim.x / G, gt = threadIdx.x % G, slot = threadIdx.x / G;
     const float inv_d = 1.f / float(p.D);
     RowSum row_sum(red, G);
-    float w[EPT], qw[EPT], d_w[WIDE ? 1 : 2][EPT] = {};         // w: scale and post_weight in one
+    float w[EPT], qw[EPT], d_w[WIDE || !PRE ? 1 : 2][EPT] = {};         // w: scale and post_weight in one
     const auto load_w = [&] {
         load_weight<T, ALIGNED>(p.post_w, p.w_dtype, gt, G, p.D, 1.f, w);
         load_weight<T, ALIGNED>(p.scale, p.w_dtype, gt, G, p.D, p.scale_value, qw);
@@ -371,19 +378,23 @@ __global__ void __launch_bounds__(WIDE ? NORM_THREADS : NORM_NARROW) norm_backwa
     };
     if (!WIDE) {
         load_w();
-        load_weight<T, ALIGNED>(p.pre_w, p.w_dtype, gt, G, p.D, 1.f, qw);
+        if (PRE) load_weight<T, ALIGNED>(p.pre_w, p.w_dtype, gt, G, p.D, 1.f, qw);
     } else if (p.partial) {
         for (int i = 0; i < 2 * EPT; ++i) sums[i * blockDim.x + threadIdx.x] = 0.f;
     }
     // the ring lies behind the sums where these are kept from the start, and in their place else
-    RowRing<T, 5> ring(p, dynamic + (WIDE && p.partial ? 2 * EPT * blockDim.x * 4 : 0), bar, &gave_up, slots);
+    RowRing<T, PRE ? 5 : 3> ring(p, dynamic + (WIDE && p.partial ? 2 * EPT * blockDim.x * 4 : 0), bar, &gave_up, slots);
     if (RING) {
-        ring.src[0] = p.x; ring.src[1] = p.residual; ring.src[2] = p.gate; ring.src[3] = p.d_hidden; ring.src[4] = p.d_normed;
-        ring.stride[0] = p.x_s; ring.stride[1] = p.r_s; ring.stride[2] = p.g_s; ring.stride[3] = p.dh_s; ring.stride[4] = p.dy_s;
+        ring.src[0] = p.x; ring.src[1] = p.gate; ring.src[2] = p.d_hidden;
+        ring.stride[0] = p.x_s; ring.stride[1] = p.g_s; ring.stride[2] = p.dh_s;
+        if (PRE) {
+            ring.src[PRE ? 3 : 0] = p.d_normed ? p.residual : nullptr; ring.src[PRE ? 4 : 0] = p.d_normed;
+            ring.stride[PRE ? 3 : 0] = p.r_s; ring.stride[PRE ? 4 : 0] = p.dy_s;
+        }
         ring.init();
     }
     const auto add = [&](int which, int i, float x) {     // post and scale, pre
-        if (!WIDE) d_w[WIDE ? 0 : which][i] += x;
+        if (!WIDE) d_w[WIDE || !PRE ? 0 : which][i] += x;
         else if (p.partial) sums[(which * EPT + i) * blockDim.x + threadIdx.x] += x;
     };
     for (int64_t first = int64_t(blockIdx.x) * slots; first < p.rows; first += int64_t(gridDim.x) * slots) {
@@ -394,18 +405,22 @@ __global__ void __launch_bounds__(WIDE ? NORM_THREADS : NORM_NARROW) norm_backwa
             ring.arrive();
             if (live) {
                 ring.read(0, slot, gt, G, x);
-                if (p.residual) ring.read(1, slot, gt, G, h);
-                if (p.gate) ring.read(2, slot, gt, G, z);
-                if (p.d_hidden) ring.read(3, slot, gt, G, dh);
-                if (p.d_normed) ring.read(4, slot, gt, G, dy);
+                if (p.gate) ring.read(1, slot, gt, G, z);
+                if (p.d_hidden) ring.read(2, slot, gt, G, dh);
+                if (PRE && p.d_normed) {
+                    if (p.residual) ring.read(3, slot, gt, G, h);
+                    ring.read(4, slot, gt, G, dy);
+                }
             }
             ring.release();
         } else if (live) {
             load_row<T, ALIGNED>(p.x, row * p.x_s, gt, G, p.D, x);
-            if (p.residual) load_row<T, ALIGNED>(p.residual, row * p.r_s, gt, G, p.D, h);
             if (p.gate) load_row<T, ALIGNED>(p.gate, row * p.g_s, gt, G, p.D, z);
             if (p.d_hidden) load_row<T, ALIGNED>(p.d_hidden, row * p.dh_s, gt, G, p.D, dh);
-            if (p.d_normed) load_row<T, ALIGNED>(p.d_normed, row * p.dy_s, gt, G, p.D, dy);
+            if (PRE && p.d_normed) {
+                if (p.residual) load_row<T, ALIGNED>(p.residual, row * p.r_s, gt, G, p.D, h);
+                load_row<T, ALIGNED>(p.d_normed, row * p.dy_s, gt, G, p.D, dy);
+            }
         }
         float rx = 1.f;
         if (p.post_w) {
@@ -428,7 +443,7 @@ __global__ void __launch_bounds__(WIDE ? NORM_THREADS : NORM_NARROW) norm_backwa
 #pragma unroll
         for (int i = 0; i < EPT; ++i) x[i] *= rx;                         // ... and the normed x
         if (WIDE) load_w();
-        if (p.d_normed) {
+        if (PRE && p.d_normed) {
 #pragma unroll
             for (int i = 0; i < EPT; ++i) h[i] += w[i] * (z[i] * x[i]);
             if (WIDE) load_weight<T, ALIGNED>(p.pre_w, p.w_dtype, gt, G, p.D, 1.f, qw);
@@ -477,7 +492,7 @@ __global__ void __launch_bounds__(WIDE ? NORM_THREADS : NORM_NARROW) norm_backwa
         if (e >= p.D) continue;
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-            const float v = WIDE ? sums[(j * EPT + i) * blockDim.x + threadIdx.x] : d_w[WIDE ? 0 : j][i];
+            const float v = WIDE ? sums[(j * EPT + i) * blockDim.x + threadIdx.x] : j == 0 || PRE ? d_w[WIDE || !PRE ? 0 : j][i] : 0.f;
             if (slots > 1) sums[(slot * 2 + j) * p.D + e] = v;
             else to[j * p.D + e] = v;
         }
@@ -552,10 +567,15 @@ static int norm_device(int *sms) {
     return ASCAN_OK;
 }
 
+// The backward without a gradient of `normed` needs neither residual nor the weights and sums of the second norm: 80 registers
+// a thread and, for rows of one CTA of 256 threads, three CTAs an SM (262144
+// heads of 128, bf16: 85 us, 101 in the general form).
+static bool lean(const NormParams &p) { return !p.d_normed && p.D <= 1024; }
+
 // Stages of the ring: at most four, in what two CTAs of an SM share (the long rows' kernels, one or two CTAs an SM) or
 // three; none where two do not fit, or where no CTA comes to a second turn.  `kept`: bytes of the sums that live beside it.
 static int ring_stages(const NormParams &p, int inputs, int slots, int grid, bool short_forward, size_t size, size_t kept) {
-    const size_t buffer = size_t(inputs) * slots * p.D * size, room = short_forward ? 48 * 1024 : 104 * 1024;
+    const size_t buffer = size_t(inputs) * slots * p.D * size, room = short_forward ? 68 * 1024 : 104 * 1024;
     if (p.rows <= int64_t(grid) * slots) return 0;
     int n = 4;
     while (n > 1 && kept + n * buffer > room) --n;
@@ -571,16 +591,17 @@ static int launch_norm(K kernel, const NormParams &p, int grid, int threads, siz
     return cudaGetLastError() == cudaSuccess ? ASCAN_OK : ASCAN_ERR_LAUNCH;
 }
 
-template <class T, bool ALIGNED, bool WIDE>
+template <class T, bool ALIGNED, int FORM>
 static int launch_back(NormParams p, int grid, int threads, cudaStream_t st) {
+    constexpr bool WIDE = FORM == WIDE_ROWS;
     const int slots = threads / p.groups;
     size_t sums = 0;
     if (p.partial) sums = WIDE ? size_t(2) * 8 * threads * 4 : slots > 1 ? size_t(slots) * 2 * p.D * 4 : 0;   // at most 64 KB
-    p.stages = ALIGNED ? ring_stages(p, 5, slots, grid, false, sizeof(T), WIDE ? sums : 0) : 0;
-    const size_t ring = size_t(p.stages) * 5 * slots * p.D * sizeof(T);
+    p.stages = ALIGNED ? ring_stages(p, FORM == LEAN ? 3 : 5, slots, grid, FORM == LEAN, sizeof(T), WIDE ? sums : 0) : 0;
+    const size_t ring = size_t(p.stages) * (FORM == LEAN ? 3 : 5) * slots * p.D * sizeof(T);
     const size_t smem = WIDE ? sums + ring : sums > ring ? sums : ring;
-    if (ALIGNED && p.stages) return launch_norm(norm_backward_kernel<T, ALIGNED, WIDE, ALIGNED>, p, grid, threads, smem, st);
-    return launch_norm(norm_backward_kernel<T, ALIGNED, WIDE, false>, p, grid, threads, smem, st);
+    if (ALIGNED && p.stages) return launch_norm(norm_backward_kernel<T, ALIGNED, FORM, ALIGNED>, p, grid, threads, smem, st);
+    return launch_norm(norm_backward_kernel<T, ALIGNED, FORM, false>, p, grid, threads, smem, st);
 }
 
 template <class T, bool ALIGNED, int E>
@@ -596,8 +617,9 @@ template <class T>
 static int launch_type(const NormParams &p, int grid, int threads, bool aligned, bool backward, cudaStream_t st) {
     if (backward) {
         if (threads > NORM_NARROW)
-            return aligned ? launch_back<T, true, true>(p, grid, threads, st) : launch_back<T, false, true>(p, grid, threads, st);
-        return aligned ? launch_back<T, true, false>(p, grid, threads, st) : launch_back<T, false, false>(p, grid, threads, st);
+            return aligned ? launch_back<T, true, WIDE_ROWS>(p, grid, threads, st) : launch_back<T, false, WIDE_ROWS>(p, grid, threads, st);
+        if (lean(p)) return aligned ? launch_back<T, true, LEAN>(p, grid, threads, st) : launch_back<T, false, LEAN>(p, grid, threads, st);
+        return aligned ? launch_back<T, true, MIDDLE>(p, grid, threads, st) : launch_back<T, false, MIDDLE>(p, grid, threads, st);
     }
     if (p.D > 1024) return aligned ? launch_fore<T, true, 16>(p, grid, threads, st) : launch_fore<T, false, 16>(p, grid, threads, st);
     return aligned ? launch_fore<T, true, 8>(p, grid, threads, st) : launch_fore<T, false, 8>(p, grid, threads, st);
@@ -671,7 +693,7 @@ size_t ascan_norm_backward_bytes(const ascan_norm *a) {
         sms = 148;          // no device to ask: size for a full B200
     }
     norm_shape(p.D, 8, &p.groups, &threads);
-    return size_t(norm_grid(p.rows, p.groups, threads, sms, false)) * 2 * p.D * 4;
+    return size_t(norm_grid(p.rows, p.groups, threads, sms, p.D <= 1024)) * 2 * p.D * 4;
 }
 
 int ascan_norm_backward(const ascan_norm *a, const void *d_hidden, int64_t d_hidden_stride, const void *d_normed, int64_t d_normed_stride,
@@ -698,7 +720,7 @@ int ascan_norm_backward(const ascan_norm *a, const void *d_hidden, int64_t d_hid
     int sms = 0, threads;
     if ((rc = norm_device(&sms)) != ASCAN_OK) return rc;
     norm_shape(p.D, 8, &p.groups, &threads);
-    const int grid = norm_grid(p.rows, p.groups, threads, sms, false);
+    const int grid = norm_grid(p.rows, p.groups, threads, sms, lean(p));
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (p.rows > 0 && (rc = launch_norm_by_type(p, a->dtype, grid, threads, aligned, true, st)) != ASCAN_OK) return rc;
     if (weights) {         // without rows: zeros

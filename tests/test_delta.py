@@ -397,11 +397,11 @@ def test_step(cuda_device, shape, dtype):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("H", [2, 128])                    # few states, and more than the SMs hold at once
-def test_step_padded_rows_and_bad_slots(cuda_device, H):
+@pytest.mark.parametrize("H,V", [(2, 64), (128, 64), (128, 96)])     # few states, and more than the SMs hold at once
+def test_step_padded_rows_and_bad_slots(cuda_device, H, V):
     B = 6
-    args = token_inputs(1, B, 1, H, 64, 64, torch.bfloat16, cuda_device)
-    pool = torch.randn(4, H, 64, 64, device=cuda_device)
+    args = token_inputs(1, B, 1, H, 64, V, torch.bfloat16, cuda_device)
+    pool = torch.randn(4, H, 64, V, device=cuda_device)
     state = pool.clone()
     slots = torch.tensor([2, -1, 0, 2, 4, 1 << 30], dtype=torch.int32, device=cuda_device)
     out = delta.step(*args, state, slots)
