@@ -16,7 +16,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OUT = os.path.join(HERE, "accelerated_scan", "libascan_b200.so")
 SOURCES = ["api.cu", "planner.cpp", "inst_f32.cu", "inst_bf16.cu", "inst_f16.cu", "inst_c64.cu",
-           "delta.cu", "delta_forward.cu", "delta_forward_tc.cu", "delta_backward.cu", "delta_backward_tc.cu", "delta_grads_tc.cu",
+           "delta.cu", "delta_forward.cu", "delta_forward_tc.cu", "delta_backward.cu", "delta_backward_tc.cu",
            "norm.cu"]
 HEADERS = sorted(f for f in os.listdir(CSRC) if f.endswith((".cuh", ".h"))) + [
     os.path.join("..", "..", "include", "ascan_b200.h")]

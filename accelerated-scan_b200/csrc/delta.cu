@@ -150,7 +150,8 @@ static void fill_back(const ascan_delta *a, DeltaParams &p, Bump &bump, const vo
     const int nt = terms(a->dtype), kp = p.Kp <= 64 ? 64 : 128;
     p.dS = bump.take<__nv_bfloat16>(each * nt * p.Vp * kp);
     p.z = bump.take<__nv_bfloat16>(each * 2 * 64 * p.Vp);
-    if (!tensor_core_path(a)) take_chunks(p, bump);
+    if (tensor_core_path(a)) p.done = bump.take<int>(2 + each);
+    else take_chunks(p, bump);
     plan_pack(a, d_out, d_out_stride, a->heads, a->v_dim, &p.d_out, bump, jobs, n_jobs);
 }
 
@@ -553,10 +554,7 @@ int ascan_delta_backward(const ascan_delta *a, const void *d_out, const int64_t 
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if ((rc = run_packs(a, jobs, n, st)) != ASCAN_OK) return rc;
     if ((rc = delta_launch_zero_outside(p, st)) != ASCAN_OK) return rc;
-    if (tensor_core_path(a)) {
-        if ((rc = delta_launch_back_sweep_tc(p, st)) != ASCAN_OK) return rc;
-        return delta_launch_grads_tc(p, sms, st);
-    }
+    if (tensor_core_path(a)) return delta_launch_backward_tc(p, sms, st);
     if ((rc = delta_launch_prep(p, st)) != ASCAN_OK) return rc;
     if ((rc = delta_launch_back_sweep(p, sms, st)) != ASCAN_OK) return rc;
     return delta_launch_grads(p, st);

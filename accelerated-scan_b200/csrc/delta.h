@@ -49,6 +49,7 @@ struct DeltaParams {
     __nv_bfloat16 *S, *e;            // saved for the backward: [slot][H][nt][Vp][KP] and [slot][H][nt][Vp][64]
     // backward
     __nv_bfloat16 *dS, *z;           // as S and e
+    int *done;                       // two tickets, and [slot][H]: slices of V that the sweep has finished
     const float *d_s1;
     float *d_s0;
     void *d_q, *d_k, *d_v, *d_g, *d_b;
@@ -60,10 +61,9 @@ int delta_launch_pack(const void *src, int dtype, const int64_t *strides, int64_
 int delta_launch_prep(const DeltaParams &p, cudaStream_t st);
 int delta_launch_sweep(const DeltaParams &p, bool save, int sm_count, cudaStream_t st);
 int delta_launch_sweep_tc(const DeltaParams &p, bool save, cudaStream_t st);
-int delta_launch_back_sweep_tc(const DeltaParams &p, cudaStream_t st);
+int delta_launch_backward_tc(const DeltaParams &p, int sm_count, cudaStream_t st);
 int delta_launch_back_sweep(const DeltaParams &p, int sm_count, cudaStream_t st);
 int delta_launch_zero_outside(const DeltaParams &p, cudaStream_t st);
 int delta_launch_grads(const DeltaParams &p, cudaStream_t st);
-int delta_launch_grads_tc(const DeltaParams &p, int sm_count, cudaStream_t st);
 
 }  // namespace ascan

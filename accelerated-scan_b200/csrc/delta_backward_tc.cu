@@ -3,10 +3,11 @@
 //     du = Gam_C (dS^T K^T) + d_out^T P;   z = du - du (beta M);   y = beta z = dV
 //     dS^T = gam_C dS^T + (scale gam d_out)^T Q - (gam y)^T K
 // d_out^T P takes d_out from shared memory as it is (rows of the product lie along the tile's rows); it and
-// (scale gam d_out)^T Q do not wait for the state and run while the threads convert.  dS1 and z go to memory for the kernel
-// that follows.  M and P are prepared again: reading them back would be 32 KB a chunk and head, and the groups that prepare
-// would idle.  Bound as the forward sweep is; 4 x 4096 tokens, 16 heads of 128 x 128: 413 us.
-#include "delta_tc_roles.cuh"
+// (scale gam d_out)^T Q do not wait for the state and run while the threads convert.  dS1 and z go to memory for the gradients
+// of the chunk, which other CTAs of the same launch compute meanwhile.  M and P are prepared again: reading them back would be 32 KB a chunk and head, and the groups that prepare
+// would idle.  Bound as the forward sweep is; 4 x 4096 tokens, 16 heads of 128 x 128: 413 us by itself,
+// and 489 with the gradients beside it, whose 266 us by themselves would else come behind.
+#include "delta_grads_tc.cuh"
 
 namespace ascan {
 
@@ -16,13 +17,11 @@ struct TcBackward {          // columns of tensor memory; A1 lies in D2's place,
 enum : int { B_D1 = B_OWN, B_D2, B_D3, B_S, B_AS, B_DU, B_A1, B_YZ };
 
 template <int KP>
-__global__ void __launch_bounds__(TC_THREADS, 1) delta_back_sweep_tc_kernel(const __grid_constant__ DeltaParams p,
-                                                                            const __grid_constant__ TcMaps maps) {
-    extern __shared__ unsigned char smem_raw[];
+__device__ __forceinline__ void back_sweep(const DeltaParams &p, const TcMaps &maps, unsigned char *smem_raw, int block) {
     typedef TcLayout<KP, true> L;
     typedef TcBackward F;
     constexpr int HK = KP / 2;                         // columns of the state a thread holds
-    const TcBlock k = tc_begin<L>(p, smem_raw, 4, 4);
+    const TcBlock k = tc_begin<L>(p, smem_raw, block, 4, 4);
     const Sequence &sq = k.sq;
     unsigned char *smem = k.smem;
     const uint32_t base = k.base, tmem = k.tmem;
@@ -263,25 +262,46 @@ __global__ void __launch_bounds__(TC_THREADS, 1) delta_back_sweep_tc_kernel(cons
     tc_end(k);
 }
 
-template <int KP>
-static int launch_back_sweep_tc(const DeltaParams &p, const TcMaps &maps, cudaStream_t st) {
-    const int64_t grid = int64_t(p.n_seqs) * p.H * ((p.Vp + 127) / 128);
-    const int smem = TcLayout<KP, true>::BYTES;
-    if (grid > 0x7fffffff) return ASCAN_ERR_UNSUPPORTED;
-    if (cudaFuncSetAttribute(delta_back_sweep_tc_kernel<KP>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
-        return ASCAN_ERR_LAUNCH;
-    delta_back_sweep_tc_kernel<KP><<<unsigned(grid), TC_THREADS, smem, st>>>(p, maps);
+// The sweep and the gradients of the chunks that it has finished, in one launch: the first `sweeps` CTAs to start sweep, so a
+// CTA that waits for a sweep waits for one that runs.  One sweep needs one SM a head and sequence, and leaves the others idle.
+template <int KP, bool GROUPED>
+__global__ void __launch_bounds__(TC_THREADS, 1) delta_backward_tc_kernel(const __grid_constant__ DeltaParams p, const __grid_constant__ TcMaps maps,
+                                                                          const __grid_constant__ GradMaps grad_maps, int sweeps) {
+    extern __shared__ unsigned char smem_raw[];
+    volatile int *ticket = reinterpret_cast<volatile int *>(smem_raw);
+    if (threadIdx.x == 0) *ticket = atomicAdd(p.done, 1);
+    __syncthreads();
+    const int role = *ticket;
+    __syncthreads();
+    if (role < sweeps) back_sweep<KP>(p, maps, smem_raw, role);
+    else chunk_gradients<GROUPED>(p, grad_maps, smem_raw);
+}
+
+template <int KP, bool GROUPED>
+static int launch_backward_tc(const DeltaParams &p, const TcMaps &maps, const GradMaps &grad_maps, int sm_count, cudaStream_t st) {
+    const int64_t sweeps = int64_t(p.n_seqs) * p.H * ((p.Vp + 127) / 128), items = int64_t(p.slots) * p.Hk;
+    const int64_t others = items < sm_count ? items : sm_count;
+    if (sweeps + others > 0x7fffffff) return ASCAN_ERR_UNSUPPORTED;
+    const int smem = TcLayout<KP, true>::BYTES > TcGrads::BYTES ? TcLayout<KP, true>::BYTES : TcGrads::BYTES;
+    const auto kernel = delta_backward_tc_kernel<KP, GROUPED>;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return ASCAN_ERR_LAUNCH;
+    if (cudaMemsetAsync(p.done, 0, (2 + size_t(p.slots) * p.H) * sizeof(int), st) != cudaSuccess) return ASCAN_ERR_LAUNCH;
+    kernel<<<unsigned(sweeps + others), TC_THREADS, smem, st>>>(p, maps, grad_maps, static_cast<int>(sweeps));
     return cudaGetLastError() == cudaSuccess ? ASCAN_OK : ASCAN_ERR_LAUNCH;
 }
 
-int delta_launch_back_sweep_tc(const DeltaParams &p, cudaStream_t st) {
+int delta_launch_backward_tc(const DeltaParams &p, int sm_count, cudaStream_t st) {
     TcMaps maps;
+    GradMaps grad_maps;
     int rc;
     if ((rc = make_map(&maps.k, p.k, p, p.Kp, p.Hk, 64, true)) != ASCAN_OK) return rc;
     if ((rc = make_map(&maps.q, p.q, p, p.Kp, p.Hk, 64, true)) != ASCAN_OK) return rc;
     if ((rc = make_map(&maps.v, p.d_out, p, p.Vp, p.H, 64, true)) != ASCAN_OK) return rc;
     if ((rc = make_store_map(&maps, p.d_v, p, true)) != ASCAN_OK) return rc;
-    return p.Kp <= 64 ? launch_back_sweep_tc<64>(p, maps, st) : launch_back_sweep_tc<128>(p, maps, st);
+    if ((rc = make_grad_maps(&grad_maps, p)) != ASCAN_OK) return rc;
+    const bool grouped = p.H != p.Hk;
+    if (p.Kp <= 64) return grouped ? launch_backward_tc<64, true>(p, maps, grad_maps, sm_count, st) : launch_backward_tc<64, false>(p, maps, grad_maps, sm_count, st);
+    return grouped ? launch_backward_tc<128, true>(p, maps, grad_maps, sm_count, st) : launch_backward_tc<128, false>(p, maps, grad_maps, sm_count, st);
 }
 
 }  // namespace ascan

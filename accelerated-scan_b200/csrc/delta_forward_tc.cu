@@ -32,7 +32,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) delta_sweep_tc_kernel(const __g
     typedef TcLayout<KP, false> L;
     typedef TcForward F;
     constexpr int HK = KP / 2;                         // columns of the state a thread holds
-    const TcBlock k = tc_begin<L>(p, smem_raw, 4, 5);
+    const TcBlock k = tc_begin<L>(p, smem_raw, blockIdx.x, 4, 5);
     const Sequence &sq = k.sq;
     unsigned char *smem = k.smem;
     const uint32_t base = k.base, tmem = k.tmem;

@@ -10,8 +10,12 @@
 // A persistent CTA walks over (chunk, key head) and the value heads of each; V comes in slabs of 64 through a ring of two, so
 // that copies go on while D, F and the sums are worked on.  16 warps: thread (row, quarter of the columns) holds 16 values of
 // every product.  What bounds it is the chain of an item, products - D, F - products - sums - stores, which one CTA an SM cannot
-// hide: 4 x 4096 tokens, 16 heads of 128 x 128 take 266 us for 600 MB (2.3 TB/s); the mma.sync kernel took 397 there, and 486
-// went to the first form of this one (8 warps, <S0, dS1> re-read from memory, an exponential an element of D and F).
+// hide: 4 x 4096 tokens, 16 heads of 128 x 128 took 266 us for 600 MB (2.3 TB/s) as a kernel of its own; on mma.sync 397, and
+// with 8 warps, <S0, dS1> re-read from memory and an exponential an element of D and F 486.  It runs beside the sweep, on the
+// SMs that the sweep leaves and on all of them behind it: the two take 489 us, not 679; with the chunks dealt out in advance
+// over the SMs that do not sweep 590.
+#pragma once
+
 #include "delta_tc_roles.cuh"
 
 namespace ascan {
@@ -34,26 +38,51 @@ struct TcGrads {
     static constexpr int DQ1 = 0, DR1 = 64, DW1 = 128, DP = 192, F0 = 256, DQ2 = 320, DR2 = 384, DW2 = 448;
 };
 static_assert(TcGrads::BYTES <= 227 * 1024, "shared memory");
-enum : int { G_SLAB = 0, G_KQ = 2, G_ACC, G_OUT, G_TAIL, G_DF, G_READ, G_KQ_FREE, G_SLAB_FREE, G_COUNT = G_SLAB_FREE + 2 };
+enum : int { G_SLAB = 0, G_KQ = 2, G_ACC, G_OUT, G_TAIL, G_DF, G_READ, G_KQ_FREE, G_SLAB_FREE, G_ITEM = G_SLAB_FREE + 2, G_COUNT = G_ITEM + 2 };
 
-constexpr int GRADS_WARPS = 16, GRADS_COMPUTE = 32 * GRADS_WARPS, GRADS_THREADS = GRADS_COMPUTE + 64;
+constexpr int GRADS_WARPS = 16, GRADS_COMPUTE = 32 * GRADS_WARPS;      // and one that copies, one that issues
 
+// Until the sweep has finished a chunk of a head, in all its slices of V: dS1 and z are in memory then, and what the copies
+// read is what was written.  One thread.  A sweep takes about six microseconds a chunk: the limit
+// allows a second and sixty a chunk.
+__device__ __forceinline__ void wait_for_sweep(const DeltaParams &p, int at, const Waiter &wait) {
+    const int slices = (p.Vp + 127) / 128;
+    int64_t left = (int64_t(1) << 21) + 2 * p.T;
+    int seen;
+    while (true) {
+        asm volatile("ld.acquire.gpu.global.s32 %0, [%1];" : "=r"(seen) : "l"(p.done + 2 + at) : "memory");
+        if (seen >= slices || *wait.dead) break;
+        if (--left == 0) {
+            *wait.dead = 1;
+            if (wait.status) *reinterpret_cast<volatile int *>(wait.status) = 1;
+        }
+        __nanosleep(500);
+    }
+    asm volatile("fence.proxy.async.global;" ::: "memory");
+}
+
+// CTAs take chunks from a counter, in the order in which the sweep finishes them: CTAs that start when the sweeps end share what
+// is left.  The copying warp takes them, the others read them from a ring of two (an item's place is written again when K and
+// Q of the item behind it have been waited for, which all of them have finished then).
 template <bool GROUPED>
-__global__ void __launch_bounds__(GRADS_THREADS, 1) delta_grads_tc_kernel(const __grid_constant__ DeltaParams p,
-                                                                          const __grid_constant__ GradMaps maps) {
-    extern __shared__ unsigned char smem_raw[];
+__device__ __forceinline__ void chunk_gradients(const DeltaParams &p, const GradMaps &maps, unsigned char *smem_raw) {
     typedef TcGrads L;
     unsigned char *smem = smem_raw + (-smem_addr(smem_raw) & 1023);
     const uint32_t base = smem_addr(smem), bars = base + L::BARS;
     const auto bar = [&](int i) { return bars + 8 * i; };
     volatile int *dead = reinterpret_cast<volatile int *>(smem + L::BARS + 8 * G_COUNT);
+    volatile int *ring = dead + 4, *current = dead + 6;          // behind dead and the address of tensor memory
     const Waiter wait = {dead, p.status};
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int group = p.H / p.Hk, slabs = (p.Vp + 63) / 64;
-    const int64_t items = int64_t(p.slots) * p.Hk;
+    const int items = p.slots * p.Hk;
+    const auto slot_of = [&](int item) {
+        const int i = item / p.Hk;
+        return p.packed ? p.slots - 1 - i : i % p.n_seqs * p.chunks + p.chunks - 1 - i / p.n_seqs;
+    };
     if (tid == 0) {
         *dead = 0;
-        for (int i = 0; i < G_COUNT; ++i) mbar_init(bar(i), i < G_DF ? 1 : i < G_SLAB_FREE ? GRADS_WARPS : GRADS_WARPS + 1);
+        for (int i = 0; i < G_COUNT; ++i) mbar_init(bar(i), i < G_DF || i >= G_ITEM ? 1 : i < G_SLAB_FREE ? GRADS_WARPS : GRADS_WARPS + 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         fence_async_proxy();
     }
@@ -70,10 +99,16 @@ __global__ void __launch_bounds__(GRADS_THREADS, 1) delta_grads_tc_kernel(const 
         int n_item = 0;
         uint32_t n_head = 0, n_slab = 0;
 #pragma unroll 1
-        for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
-            const int slot = static_cast<int>(item / p.Hk), hk = static_cast<int>(item % p.Hk);
+        while (true) {
+            if (tid == 0) {                    // one thread says whether there is another item: all see the same
+                wait(bar(G_ITEM + (n_item & 1)), (n_item >> 1) & 1);
+                *current = *dead ? -1 : ring[n_item & 1];
+            }
+            sync();
+            const int item = *current;
+            if (item < 0) break;
+            const int slot = slot_of(item), hk = item % p.Hk;
             const Chunk ch = get_chunk(p, slot);
-            if (ch.rows == 0) continue;
             const int64_t tok0 = ch.b * p.T + ch.t0;
             const unsigned char *kq = smem + L::KQ + (row >> 6) * 8192 + (row & 7) * 2;
             const auto key = [&](int t, int q) {                           // K (Q) of token t, this thread's column
@@ -301,13 +336,24 @@ __global__ void __launch_bounds__(GRADS_THREADS, 1) delta_grads_tc_kernel(const 
         // ---- copies
         int n_item = 0, n_tail = 0;
         uint32_t n_slab = 0;
-        for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
-            const int slot = static_cast<int>(item / p.Hk), hk = static_cast<int>(item % p.Hk);
+        while (true) {
+            int item = 0;
+            if (lane == 0) item = *dead ? items : atomicAdd(p.done + 1, 1);
+            item = __shfl_sync(~0u, item, 0);
+            const bool more = item < items;
+            const int slot = more ? slot_of(item) : 0, hk = item % p.Hk;
             const Chunk ch = get_chunk(p, slot);
-            if (ch.rows == 0) continue;
+            if (more && ch.rows == 0) continue;
+            if (lane == 0) {
+                ring[n_item & 1] = more ? item : -1;
+                mbar_arrive(bar(G_ITEM + (n_item & 1)));
+            }
+            if (!more) break;
             const int tok = static_cast<int>(ch.t0), b0 = static_cast<int>(ch.b);
             for (int hh = 0; hh < group; ++hh) {
                 const int h = hk * group + hh, at = slot * p.H + h;
+                if (lane == 0) wait_for_sweep(p, at, wait);
+                __syncwarp();
                 for (int s = 0; s < slabs; ++s, ++n_slab) {
                     const int st = n_slab & 1;
                     if (n_slab >= 2) wait(bar(G_SLAB_FREE + st), ((n_slab - 2) >> 1) & 1);
@@ -354,7 +400,7 @@ __global__ void __launch_bounds__(GRADS_THREADS, 1) delta_grads_tc_kernel(const 
                 ++n_item;
             }
         }
-    } else if (elect_one()) {
+    } else if (warp == GRADS_WARPS + 1 && elect_one()) {
         // ---- issue.  Left operands: columns along the rows of their tiles, blocks of 64 columns 8 KB apart.  Right ones: `along`
         // a tile's rows (32 bytes a step of 16) or down them (2048).
         constexpr uint32_t ALONG = mma_desc(64, false, false, true), DOWN = mma_desc(64, true, false, true);
@@ -365,14 +411,14 @@ __global__ void __launch_bounds__(GRADS_THREADS, 1) delta_grads_tc_kernel(const 
         };
         int n_item = 0;
         uint32_t n_slab = 0, n_head = 0;
-        for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
-            const int slot = static_cast<int>(item / p.Hk);
-            if (get_chunk(p, slot).rows == 0) continue;
+        while (true) {
+            wait(bar(G_ITEM + (n_item & 1)), (n_item >> 1) & 1);
+            if (*dead || ring[n_item & 1] < 0) break;
             const uint32_t keys = base + L::KQ, queries = keys + 16384;
             for (int hh = 0; hh < group; ++hh, ++n_head) {
                 // what D and F are made of does not wait until the head before has been read; the rest does.  Both slabs of a V
                 // up to 128 stay for that; of a longer one each slab is finished in its turn.
-                const auto first = [&](uint32_t n, bool add) {
+                const auto early = [&](uint32_t n, bool add) {
                     const uint32_t d = base + (n & 1) * L::SLAB;
                     wait(bar(G_SLAB + (n & 1)), (n >> 1) & 1);
                     tc_fence_after();
@@ -396,14 +442,14 @@ __global__ void __launch_bounds__(GRADS_THREADS, 1) delta_grads_tc_kernel(const 
                     tc_fence_after();
                 };
                 if (slabs <= 2) {
-                    for (int s = 0; s < slabs; ++s) first(n_slab + s, s > 0);
+                    for (int s = 0; s < slabs; ++s) early(n_slab + s, s > 0);
                     tc_commit(bar(G_ACC));
                     read_before();
                     for (int s = 0; s < slabs; ++s) second(n_slab + s, s > 0);
                 } else {
                     read_before();
                     for (int s = 0; s < slabs; ++s) {
-                        first(n_slab + s, s > 0);
+                        early(n_slab + s, s > 0);
                         second(n_slab + s, s > 0);
                     }
                     tc_commit(bar(G_ACC));
@@ -440,22 +486,16 @@ static int scratch_map(CUtensorMap *map, const bf16 *x, const DeltaParams &p, in
     return make_box_map(map, pl, q, cols, p.Vp, 64, 64, 1, true);
 }
 
-int delta_launch_grads_tc(const DeltaParams &p, int sm_count, cudaStream_t st) {
-    if (p.slots == 0) return ASCAN_OK;
-    GradMaps maps;
+static int make_grad_maps(GradMaps *maps, const DeltaParams &p) {
     int rc;
-    if ((rc = make_map(&maps.k, p.k, p, p.Kp, p.Hk, 64, true)) != ASCAN_OK) return rc;
-    if ((rc = make_map(&maps.q, p.q, p, p.Kp, p.Hk, 64, true)) != ASCAN_OK) return rc;
-    if ((rc = make_map(&maps.d_out, p.d_out, p, p.Vp, p.H, 64, true)) != ASCAN_OK) return rc;
-    if ((rc = scratch_map(&maps.e, p.e, p, 64, 2)) != ASCAN_OK) return rc;
-    if ((rc = scratch_map(&maps.z, p.z, p, 64, 2)) != ASCAN_OK) return rc;
-    if ((rc = scratch_map(&maps.S, p.S, p, p.Kp <= 64 ? 64 : 128, 1)) != ASCAN_OK) return rc;
-    if ((rc = scratch_map(&maps.dS, p.dS, p, p.Kp <= 64 ? 64 : 128, 1)) != ASCAN_OK) return rc;
-    const auto kernel = p.H == p.Hk ? delta_grads_tc_kernel<false> : delta_grads_tc_kernel<true>;
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, TcGrads::BYTES) != cudaSuccess) return ASCAN_ERR_LAUNCH;
-    const int64_t items = int64_t(p.slots) * p.Hk;
-    kernel<<<static_cast<unsigned>(items < sm_count ? items : sm_count), GRADS_THREADS, TcGrads::BYTES, st>>>(p, maps);
-    return cudaGetLastError() == cudaSuccess ? ASCAN_OK : ASCAN_ERR_LAUNCH;
+    if ((rc = make_map(&maps->k, p.k, p, p.Kp, p.Hk, 64, true)) != ASCAN_OK) return rc;
+    if ((rc = make_map(&maps->q, p.q, p, p.Kp, p.Hk, 64, true)) != ASCAN_OK) return rc;
+    if ((rc = make_map(&maps->d_out, p.d_out, p, p.Vp, p.H, 64, true)) != ASCAN_OK) return rc;
+    if ((rc = scratch_map(&maps->e, p.e, p, 64, 2)) != ASCAN_OK) return rc;
+    if ((rc = scratch_map(&maps->z, p.z, p, 64, 2)) != ASCAN_OK) return rc;
+    if ((rc = scratch_map(&maps->S, p.S, p, p.Kp <= 64 ? 64 : 128, 1)) != ASCAN_OK) return rc;
+    if ((rc = scratch_map(&maps->dS, p.dS, p, p.Kp <= 64 ? 64 : 128, 1)) != ASCAN_OK) return rc;
+    return ASCAN_OK;
 }
 
 }  // namespace ascan

@@ -122,17 +122,17 @@ struct TcBlock {             // what every role starts from
     __device__ __forceinline__ uint32_t bar(int i) const { return bars + 8 * i; }
 };
 
-// commits: barriers from B_OWN on that one commit completes; the next `warps` ones take eight warps
+// block: which sequence, head and 128 columns of V.  commits: barriers from B_OWN on that one commit completes; the next `warps` ones take eight warps
 template <class L>
-__device__ __forceinline__ TcBlock tc_begin(const DeltaParams &p, unsigned char *raw, int commits, int warps) {
+__device__ __forceinline__ TcBlock tc_begin(const DeltaParams &p, unsigned char *raw, int block, int commits, int warps) {
     TcBlock k;
     k.smem = raw + (-smem_addr(raw) & 1023);
     k.base = smem_addr(k.smem);
     k.bars = k.base + L::BARS;
     const int slices = (p.Vp + 127) / 128, count = B_OWN + commits + warps;
-    k.v0 = blockIdx.x % slices * 128;
-    k.h = blockIdx.x / slices % p.H;
-    k.n_seq = blockIdx.x / slices / p.H;
+    k.v0 = block % slices * 128;
+    k.h = block / slices % p.H;
+    k.n_seq = block / slices / p.H;
     k.hk = k.h / (p.H / p.Hk);
     k.sq = get_sequence(p, k.n_seq);
     volatile int *dead = reinterpret_cast<volatile int *>(k.smem + L::BARS + 8 * count);
@@ -216,6 +216,14 @@ __device__ __forceinline__ void prepare_chunks(const DeltaParams &p, const TcBlo
 template <class L, bool BACK, bool V_HALVES>
 __device__ __forceinline__ void load_tiles(const DeltaParams &p, const TcBlock &k, const TcMaps &maps) {
     const int lane = threadIdx.x & 31, b0 = static_cast<int>(k.sq.b);
+    // Backward: a chunk whose tiles are free has written z and dS1; the CTAs that wait for them are told.
+    const auto publish = [&](int turn) {
+        if (lane == 0) {
+            __threadfence();
+            atomicAdd(p.done + 2 + (k.sq.slot0 + k.sq.chunks - 1 - turn) * p.H + k.h, 1);
+        }
+        __syncwarp();
+    };
 #pragma unroll 1
     for (int turn = 0; turn < k.sq.chunks; ++turn) {
         const int c = BACK ? k.sq.chunks - 1 - turn : turn, stage = turn % 3;
@@ -253,7 +261,14 @@ __device__ __forceinline__ void load_tiles(const DeltaParams &p, const TcBlock &
             __syncwarp();
             if (lane == 0) mbar_arrive(k.bar(B_TILE + stage));
         }
+        if (BACK && turn >= 3) publish(turn - 3);
     }
+    if (BACK)
+#pragma unroll 1
+        for (int turn = k.sq.chunks < 3 ? 0 : k.sq.chunks - 3; turn < k.sq.chunks; ++turn) {
+            k.wait(k.bar(B_FREE + turn % 3), (turn / 3) & 1);
+            publish(turn);
+        }
 }
 
 // Gates, as far ahead as there is room; one warp.  KEEP: also to memory, for the backward's second kernel.
