@@ -6,7 +6,7 @@
 // (scale gam d_out)^T Q do not wait for the state and run while the threads convert.  dS1 and z go to memory for the gradients
 // of the chunk, which other CTAs of the same launch compute meanwhile.  M and P are prepared again: reading them back would be 32 KB a chunk and head, and the groups that prepare
 // would idle.  Bound as the forward sweep is; 4 x 4096 tokens, 16 heads of 128 x 128: 413 us by itself,
-// and 489 with the gradients beside it, whose 266 us by themselves would else come behind.
+// and 480 with the gradients beside it, whose 266 us by themselves would else come behind.
 #include "delta_grads_tc.cuh"
 
 namespace ascan {
@@ -56,10 +56,10 @@ __device__ __forceinline__ void back_sweep(const DeltaParams &p, const TcMaps &m
             // this thread's column of the tile of d_out, and later of dV: row t, piece (v % 64) / 8 of a swizzled block
             unsigned char *col = smem + stage * L::STAGE + L::KQ_BYTES + (v >> 6) * 8192 + part * 32 * 128 + (v & 7) * 2;
             const auto element = [&](int t) { return reinterpret_cast<uint16_t *>(col + t * 128 + (((v >> 3 & 7) ^ (t & 7)) << 4)); };
-            k.wait(k.bar(B_TILE + stage), (turn / 3) & 1);
-            k.wait(k.bar(B_GATES + stage), (turn / 3) & 1);
-            k.wait(k.bar(B_D2), turn & 1);
-            k.wait(k.bar(B_D1), turn & 1);
+            k.wait.warp(k.bar(B_TILE + stage), (turn / 3) & 1);
+            k.wait.warp(k.bar(B_GATES + stage), (turn / 3) & 1);
+            k.wait.warp(k.bar(B_D2), turn & 1);
+            k.wait.warp(k.bar(B_D1), turn & 1);
             tc_fence_after();
             f2 x[16];
             {
@@ -103,7 +103,7 @@ __device__ __forceinline__ void back_sweep(const DeltaParams &p, const TcMaps &m
                 tmem_st8(t0 + F::D2 + 32 * part + 16 + 8 * q, lo);
             }
             hand_over(k, B_A1);
-            k.wait(k.bar(B_D3), turn & 1);
+            k.wait.warp(k.bar(B_D3), turn & 1);
             tc_fence_after();
             tmem_ld32(r, t0 + F::D3 + 32 * part);
             tc_wait_ld();
@@ -158,7 +158,7 @@ __device__ __forceinline__ void back_sweep(const DeltaParams &p, const TcMaps &m
             }
             const float gam_c = sc[SC_GAM * 64 + 63 - part * 32];
             const f2 gam_c2 = two(gam_c, gam_c);
-            k.wait(k.bar(B_S), turn & 1);
+            k.wait.warp(k.bar(B_S), turn & 1);
             tc_fence_after();
 #pragma unroll
             for (int q = 0; q < HK / 32; ++q) {

@@ -65,15 +65,15 @@ __global__ void __launch_bounds__(TC_THREADS, 1) delta_sweep_tc_kernel(const __g
             const float *sc = reinterpret_cast<const GateShared *>(smem + L::SC)[stage].sc + part * 32;
             const auto scalars = [&](int which, int i) { return *reinterpret_cast<const ulonglong2 *>(sc + which * 64 + i); };
             unsigned char *vt = smem + stage * L::STAGE + L::KQ_BYTES + part * 32 * 256 + v * 2;
-            k.wait(k.bar(B_TILE + stage), (c / 3) & 1);
-            k.wait(k.bar(B_GATES + stage), (c / 3) & 1);
-            k.wait(k.bar(B_PREP + (c & 1)), (c >> 1) & 1);
+            k.wait.warp(k.bar(B_TILE + stage), (c / 3) & 1);
+            k.wait.warp(k.bar(B_GATES + stage), (c / 3) & 1);
+            k.wait.warp(k.bar(B_PREP + (c & 1)), (c >> 1) & 1);
             f2 x[16];
 #pragma unroll
             for (int i = 0; i < 16; ++i)
                 x[i] = two_bits(uint32_t(*reinterpret_cast<const uint16_t *>(vt + 2 * i * 256)) << 16,
                                 uint32_t(*reinterpret_cast<const uint16_t *>(vt + (2 * i + 1) * 256)) << 16);
-            k.wait(k.bar(B_X), c & 1);
+            k.wait.warp(k.bar(B_X), c & 1);
             tc_fence_after();
             uint32_t r[32];
             tmem_ld32(r, t0 + F::X + 32 * part);
@@ -94,7 +94,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) delta_sweep_tc_kernel(const __g
                 tmem_st8(t0 + F::BX + 32 + 16 * part + 8 * q, lo);
             }
             hand_over(k, B_BX);
-            k.wait(k.bar(B_D2), c & 1);
+            k.wait.warp(k.bar(B_D2), c & 1);
             tc_fence_after();
             tmem_ld32(r, t0 + F::D2 + 32 * part);
             tc_wait_ld();
@@ -130,7 +130,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) delta_sweep_tc_kernel(const __g
             hand_over(k, B_UO);
             const float gam_c = sc[SC_GAM * 64 + 63 - part * 32];
             const f2 gam_c2 = two(gam_c, gam_c);
-            k.wait(k.bar(B_S), c & 1);
+            k.wait.warp(k.bar(B_S), c & 1);
             tc_fence_after();
 #pragma unroll
             for (int q = 0; q < HK / 32; ++q) {
@@ -145,7 +145,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) delta_sweep_tc_kernel(const __g
             }
             if (SAVE && v0 + v < p.Vp)
                 keep_tokens(x, p.e + ((int64_t(sq.slot0 + c) * p.H + h) * 2 * p.Vp + v0 + v) * 64 + 32 * part, int64_t(p.Vp) * 64);
-            k.wait(k.bar(B_O), c & 1);
+            k.wait.warp(k.bar(B_O), c & 1);
             tc_fence_after();
             uint32_t r2[32];
             tmem_ld32(r, t0 + F::O1 + 32 * part);

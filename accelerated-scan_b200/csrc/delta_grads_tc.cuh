@@ -12,7 +12,7 @@
 // every product.  What bounds it is the chain of an item, products - D, F - products - sums - stores, which one CTA an SM cannot
 // hide: 4 x 4096 tokens, 16 heads of 128 x 128 took 266 us for 600 MB (2.3 TB/s) as a kernel of its own; on mma.sync 397, and
 // with 8 warps, <S0, dS1> re-read from memory and an exponential an element of D and F 486.  It runs beside the sweep, on the
-// SMs that the sweep leaves and on all of them behind it: the two take 489 us, not 679; with the chunks dealt out in advance
+// SMs that the sweep leaves and on all of them behind it: the two take 480 us, not 679; with the chunks dealt out in advance
 // over the SMs that do not sweep 590.
 #pragma once
 
@@ -144,31 +144,27 @@ __device__ __forceinline__ void chunk_gradients(const DeltaParams &p, const Grad
                     if ((lane & 15) == 0) direct[t >> 4] = ((ok >> (lane & 16)) & 0xffffu) != 0xffffu;
                 }
                 const float gam_c = sc[SC_GAM * 64 + 63];
-                // <S0, dS1>, on the diagonals of S0 dS1^T: 16 rows of v against themselves
+                // <S0, dS1>: 16 products a thread and slab, by plain loads (as a diagonal of warp products, beside the tcgen05 products
+                // that read the same slab, it differed from run to run)
                 float dot_s = 0.f;
 #pragma unroll 1
                 for (int s = 0; s < slabs; ++s, ++n_slab) {
-                    const uint32_t d = base + (n_slab & 1) * L::SLAB;
-                    wait(bar(G_SLAB + (n_slab & 1)), (n_slab >> 1) & 1);
-                    // a warp: 16 rows (of 64) x 32 columns (of 128)
-                    const int v = 16 * (warp & 3), half = part >> 1, c0 = (part & 1) * 4;
-                    const uint32_t a0 = d + L::S + half * 8192, b0 = d + L::DS + half * 8192;
-                    float lo[4] = {}, hi[4] = {};
+                    wait.warp(bar(G_SLAB + (n_slab & 1)), (n_slab >> 1) & 1);
+                    // both lie alike: the same 16 bytes of each half of either
 #pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        uint32_t a[4], b[4];
-                        ldsm4(a, addr_an<8>(a0, v, c0 + 2 * j, lane));
-                        ldsm4(b, addr_bn<8>(b0, v, c0 + 2 * j, lane));
-                        mma(lo, a, b[0], b[1]);
-                        mma(hi, a, b[2], b[3]);
+                    for (int half = 0; half < 2; ++half) {
+                        const unsigned char *at = smem + (n_slab & 1) * L::SLAB + half * 8192 + tid * 16;
+                        const uint4 x = *reinterpret_cast<const uint4 *>(at + L::S), y = *reinterpret_cast<const uint4 *>(at + L::DS);
+                        const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) dot_s += low_half(xs[j]) * low_half(ys[j]) + high_half(xs[j]) * high_half(ys[j]);
                     }
-                    if ((lane >> 2) >> 1 == (lane & 3)) dot_s += (lane >> 2) & 1 ? lo[1] + hi[3] : lo[0] + hi[2];
                     __syncwarp();
                     if (lane == 0) mbar_arrive(bar(G_SLAB_FREE + (n_slab & 1)));
                 }
                 dot_s *= gam_c;
                 sync();
-                wait(bar(G_ACC), n_head & 1);
+                wait.warp(bar(G_ACC), n_head & 1);
                 tc_fence_after();
                 // D^T (rows j, this quarter of i) on rows 0 - 63, F (rows i, this quarter of j) on rows 64 - 127
                 {
@@ -231,8 +227,8 @@ __device__ __forceinline__ void chunk_gradients(const DeltaParams &p, const Grad
                 fence_async_proxy();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(bar(G_DF));
-                if (hh == 0) wait(bar(G_KQ), n_item & 1);
-                wait(bar(G_OUT), n_head & 1);
+                if (hh == 0) wait.warp(bar(G_KQ), n_item & 1);
+                wait.warp(bar(G_OUT), n_head & 1);
                 tc_fence_after();
                 float dot[16];
 #pragma unroll

@@ -39,6 +39,11 @@ struct Waiter {
             }
         }
     }
+    // All lanes together: they may leave the loop one by one, and what follows (ldmatrix, tcgen05.ld) needs the whole warp.
+    __device__ __forceinline__ void warp(uint32_t bar, uint32_t parity) const {
+        (*this)(bar, parity);
+        __syncwarp();
+    }
 };
 
 // Before a CTA ends: one that was given up may have copies in flight, which end by themselves within microseconds.

@@ -174,12 +174,12 @@ __device__ __forceinline__ void prepare_chunks(const DeltaParams &p, const TcBlo
 #pragma unroll 1
     for (int turn = team; turn < k.sq.chunks; turn += 2) {
         const GateShared &gs = reinterpret_cast<const GateShared *>(k.smem + L::SC)[turn % 3];
-        k.wait(k.bar(B_GATES + turn % 3), (turn / 3) & 1);
+        k.wait.warp(k.bar(B_GATES + turn % 3), (turn / 3) & 1);
         unsigned char *pt = k.smem + L::P + turn % L::P_BUFFERS * L::P_BYTES;      // three: free when this chunk's gates were written
         const float factor = !l_row ? p.scale : BACK ? gs.sc[SC_BETA * 64 + i] : 1.f;
         row_factors(f, factor, gs, i, t);
-        if (turn >= 2) k.wait(k.bar(B_MP + team), ((turn - 2) >> 1) & 1);
-        k.wait(k.bar(B_KK + team), (turn >> 1) & 1);
+        if (turn >= 2) k.wait.warp(k.bar(B_MP + team), ((turn - 2) >> 1) & 1);
+        k.wait.warp(k.bar(B_KK + team), (turn >> 1) & 1);
         tc_fence_after();
         decayed_row(row, f, factor, !BACK && l_row, !l_row, gs, i, t, [&](int bj, const float (&x)[16]) {
             if (l_row) {

@@ -633,6 +633,26 @@ def test_boundaries_outside_of_the_row_are_cut_off(cuda_device, dtype):
         assert torch.equal(a, b)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("Hk,H,V", [(4, 8, 136), (4, 4, 192), (4, 16, 128), (8, 8, 64)])
+def test_many_chunks_repeat_bit_for_bit(cuda_device, Hk, H, V, dtype):
+    """Chunks of many short sequences, which CTAs take in any order: the same bits every time."""
+    lengths = [37, 1, 64, 5, 90, 66, 0, 23] * 8
+    args = inputs(V, 1, sum(lengths), Hk, H, 128, V, dtype, cuda_device, n=len(lengths))
+    starts = torch.tensor([0] + lengths).cumsum(0).to(torch.int32).to(cuda_device)
+    leaves = [t.requires_grad_(True) for t in args]
+    first = None
+    for _ in range(12):
+        out, s = delta.scan(*args, seq_starts=starts)
+        if first is None:
+            d_out, d_s = torch.randn_like(out), torch.randn_like(s)
+        got = (out, s, *torch.autograd.grad([out, s], leaves, [d_out, d_s]))
+        first = first or got
+        for a, b in zip(got, first):
+            assert torch.equal(a, b)
+
+
 def test_an_expired_wait_is_reported_once(monkeypatch):
     """The word that a kernel sets when it gives up is read, and cleared, by the next call on its device."""
     from accelerated_scan import _native
