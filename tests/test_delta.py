@@ -653,6 +653,28 @@ def test_many_chunks_repeat_bit_for_bit(cuda_device, Hk, H, V, dtype):
             assert torch.equal(a, b)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_training_steps_on_two_streams_at_once(cuda_device, dtype):
+    """Kernels of two calls share the GPU: neither waits for the other, and each has its own scratch."""
+    calls = [inputs(40 + i, 4, 700, 4, 8, 128, 128, dtype, cuda_device) for i in range(2)]
+    leaves = [[t.requires_grad_(True) for t in args] for args in calls]
+    d = [torch.randn(4, 700, 8, 128, device=cuda_device).to(dtype) for _ in calls]
+    want = [torch.autograd.grad(delta.scan(*args)[0], own, g) for args, own, g in zip(calls, leaves, d)]
+    streams = [torch.cuda.Stream() for _ in calls]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(4):
+        for i, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                got[i].append(torch.autograd.grad(delta.scan(*calls[i])[0], leaves[i], d[i]))
+    torch.cuda.synchronize()
+    for own, expected in zip(got, want):
+        for grads in own:
+            for a, b in zip(grads, expected):
+                assert torch.equal(a, b)
+
+
 def test_an_expired_wait_is_reported_once(monkeypatch):
     """The word that a kernel sets when it gives up is read, and cleared, by the next call on its device."""
     from accelerated_scan import _native
