@@ -46,7 +46,7 @@ struct DeltaParams {
     // scratch
     __nv_bfloat16 *M, *P;            // [slot][H][2][64][64]
     float *sc;                       // [slot][H][SC_ARRAYS][64]
-    __nv_bfloat16 *S, *e;            // saved for the backward: [slot][H][nt][Vp][KP] and [slot][H][nt][Vp][64]
+    __nv_bfloat16 *S, *e;            // saved for the backward: [slot][H][terms][Vp][KP] (bf16: one term) and [slot][H][2][Vp][64]
     // backward
     __nv_bfloat16 *dS, *z;           // as S and e
     int *done;                       // two tickets, and [slot][H]: slices of V that the sweep has finished

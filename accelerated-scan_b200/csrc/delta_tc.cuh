@@ -1,5 +1,5 @@
 // Fifth-generation tensor core path of the gated delta rule: mbarriers with bounded waits, tcgen05 wrappers, and the
-// warpgroup that prepares a chunk (gates, M, P) while others carry the state through the chunk before it.
+// arithmetic of a chunk that is prepared (gates, M, P) while others carry the state through the chunk before it.
 #pragma once
 
 #include "delta_common.cuh"

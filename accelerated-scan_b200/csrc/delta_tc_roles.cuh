@@ -271,7 +271,7 @@ __device__ __forceinline__ void load_tiles(const DeltaParams &p, const TcBlock &
         }
 }
 
-// Gates, as far ahead as there is room; one warp.  KEEP: also to memory, for the backward's second kernel.
+// Gates, as far ahead as there is room; one warp.  KEEP: also to memory, for the gradients of the chunk.
 template <class L, bool BACK, bool KEEP>
 __device__ __forceinline__ void run_gates(const DeltaParams &p, const TcBlock &k) {
     const int lane = threadIdx.x & 31;
