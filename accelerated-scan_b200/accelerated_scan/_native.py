@@ -55,7 +55,7 @@ class Delta(ctypes.Structure):
                 + [("batch", _I64), ("seqlen", _I64)]
                 + [(n, _I32) for n in ("heads_k", "heads", "k_dim", "v_dim", "dtype", "log_gates_dtype", "betas_dtype")]
                 + [("scale", ctypes.c_float), ("initial_state", _PTR), ("seq_starts", _PTR), ("n_seqs", _I32),
-                   ("seq_starts_64", _I32), ("status", _PTR)])
+                   ("seq_starts_64", _I32), ("kept_packed", _I32), ("status", _PTR)])
 
 
 class DeltaToken(ctypes.Structure):
@@ -132,6 +132,8 @@ def _load():
     lib.ascan_peer_free.argtypes = [vp]
     lib.ascan_delta_forward_bytes.restype = sz
     lib.ascan_delta_forward_bytes.argtypes = [vp, i32]
+    lib.ascan_delta_packed.restype = i32
+    lib.ascan_delta_packed.argtypes = [vp]
     lib.ascan_delta_forward.restype = i32
     lib.ascan_delta_forward.argtypes = [vp, vp, vp, i32, vp, sz, vp]
     lib.ascan_delta_backward_bytes.restype = sz
@@ -163,7 +165,7 @@ EXPORTS = (
     "ascan_forward_sigmoid_gates", "ascan_backward_sigmoid_gates", "ascan_backward_complex_real_tokens",
     "ascan_check_no_alloc", "ascan_set_option", "ascan_get_option",
     "ascan_exchange_bytes", "ascan_workspace_bytes_time_sharded", "ascan_forward_time_sharded",
-    "ascan_delta_forward_bytes", "ascan_delta_forward", "ascan_delta_backward_bytes", "ascan_delta_backward",
+    "ascan_delta_forward_bytes", "ascan_delta_packed", "ascan_delta_forward", "ascan_delta_backward_bytes", "ascan_delta_backward",
     "ascan_delta_step", "ascan_norm_forward", "ascan_norm_backward_bytes", "ascan_norm_backward",
     "ascan_backward_time_sharded", "ascan_peer_alloc", "ascan_peer_open", "ascan_peer_close", "ascan_peer_free",
 )
@@ -526,15 +528,16 @@ def _sink(device):
 
 
 # The argument structures as bytes: one packing call costs a tenth of filling a ctypes.Structure field by field.
-_DELTA = struct.Struct("@5P15q2q7ifPPiiP")
+_DELTA = struct.Struct("@5P15q2q7ifPPiiiP")
 _TOKEN = struct.Struct("@5P10qq7ifP")
 _NORM = struct.Struct("@6P4q4i2fP")
 _STRIDES = struct.Struct("@3q")
 assert (_DELTA.size, _TOKEN.size, _NORM.size) == tuple(map(ctypes.sizeof, (Delta, DeltaToken, Norm)))
 
 
-def delta_args(queries, keys, values, log_gates, betas, initial_state, scale, seq_starts) -> bytes:
-    """ascan_delta of (B, T, heads, dim) tensors with a dense last dimension, in their own strides."""
+def delta_args(queries, keys, values, log_gates, betas, initial_state, scale, seq_starts, kept_packed=0) -> bytes:
+    """ascan_delta of (B, T, heads, dim) tensors with a dense last dimension, in their own strides.  kept_packed: of a backward,
+    what its forward returned."""
     B, T, heads_k, K = queries.shape
     _, _, heads, V = values.shape
     packed = seq_starts is not None
@@ -543,11 +546,11 @@ def delta_args(queries, keys, values, log_gates, betas, initial_state, scale, se
         *queries.stride()[:3], *keys.stride()[:3], *values.stride()[:3], *log_gates.stride(), *betas.stride(),
         B, T, heads_k, heads, K, V, DTYPE_CODE[queries.dtype], DTYPE_CODE[log_gates.dtype], DTYPE_CODE[betas.dtype], scale,
         0 if initial_state is None else initial_state.data_ptr(), seq_starts.data_ptr() if packed else 0,
-        seq_starts.shape[0] - 1 if packed else 0, packed and seq_starts.dtype == torch.int64, _sink(queries.device))
+        seq_starts.shape[0] - 1 if packed else 0, packed and seq_starts.dtype == torch.int64, kept_packed, _sink(queries.device))
 
 
 def delta_forward(args: bytes, device, out, final_state, keep: bool):
-    """Returns the scratch, which holds what `delta_backward` needs when keep."""
+    """Returns the scratch, which holds what `delta_backward` needs when keep, and which inputs' copies it holds as well."""
     stream = _raw_stream(device)
     with _device_guard(device):
         nbytes = lib.ascan_delta_forward_bytes(args, keep)
@@ -556,7 +559,7 @@ def delta_forward(args: bytes, device, out, final_state, keep: bool):
         ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
         rc = lib.ascan_delta_forward(args, out.data_ptr(), final_state.data_ptr(), keep, ws.data_ptr(), nbytes, stream)
     _launched(rc, "ascan_delta_forward")
-    return ws
+    return ws, lib.ascan_delta_packed(args) if keep else 0
 
 
 def delta_backward(args: bytes, device, d_out, d_final_state, grads, d_initial_state, kept):

@@ -60,11 +60,11 @@ def _forward(queries, keys, values, log_gates, betas, initial_state, scale, seq_
     n = B if seq_starts is None else seq_starts.shape[0] - 1
     out = torch.empty(B, T, H, V, dtype=values.dtype, device=values.device)
     state = torch.empty(n, H, K, V, dtype=torch.float32, device=values.device)
-    kept = None
+    kept, packed = None, 0
     if n:
         args = _native.delta_args(queries, keys, values, log_gates, betas, initial_state, scale, seq_starts)
-        kept = _native.delta_forward(args, values.device, out, state, keep)
-    return out, state, kept
+        kept, packed = _native.delta_forward(args, values.device, out, state, keep)
+    return out, state, kept, packed
 
 
 class DeltaScan(torch.autograd.Function):
@@ -72,9 +72,9 @@ class DeltaScan(torch.autograd.Function):
     def forward(ctx, queries, keys, values, log_gates, betas, initial_state, scale, seq_starts):
         queries, keys, values = _dense_last(queries), _dense_last(keys), _dense_last(values)
         s0 = None if initial_state is None else initial_state.float().contiguous()
-        out, state, kept = _forward(queries, keys, values, log_gates, betas, s0, scale, seq_starts, True)
+        out, state, kept, packed = _forward(queries, keys, values, log_gates, betas, s0, scale, seq_starts, True)
         ctx.save_for_backward(queries, keys, values, log_gates, betas, s0, seq_starts, kept)
-        ctx.scale = scale
+        ctx.scale, ctx.packed = scale, packed
         ctx.state_dtype = None if initial_state is None else initial_state.dtype
         ctx.set_materialize_grads(False)
         return out, state
@@ -83,6 +83,9 @@ class DeltaScan(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, d_out, d_state):
         queries, keys, values, log_gates, betas, s0, seq_starts, kept = ctx.saved_tensors
+        # saved-tensor hooks may hand back equal tensors that lie in memory in another way
+        queries, keys, values = _dense_last(queries), _dense_last(keys), _dense_last(values)
+        s0 = None if s0 is None else s0.contiguous()
         if d_out is None:
             d_out = torch.zeros((), dtype=values.dtype, device=values.device).expand(values.shape)
         d_out = _dense_last(d_out)
@@ -92,7 +95,7 @@ class DeltaScan(torch.autograd.Function):
         if s0 is not None and ctx.needs_input_grad[5]:
             d_s0 = torch.empty_like(s0)
         if kept is not None:
-            args = _native.delta_args(queries, keys, values, log_gates, betas, s0, ctx.scale, seq_starts)
+            args = _native.delta_args(queries, keys, values, log_gates, betas, s0, ctx.scale, seq_starts, ctx.packed)
             _native.delta_backward(args, values.device, d_out, d_state, grads, d_s0, kept)
         if d_s0 is not None:
             d_s0 = d_s0.to(ctx.state_dtype)

@@ -73,17 +73,21 @@ static Planes user_plane(const void *p, const int64_t *s) {
     return Planes{static_cast<const __nv_bfloat16 *>(p), 0, s[0], s[1], s[2]};
 }
 
+static void take_copy(const ascan_delta *a, int heads, int d, Planes *to, Bump &bump) {
+    const int dp = round_up8(d);
+    const int64_t plane = a->batch * a->seqlen * heads * dp;
+    __nv_bfloat16 *dst = bump.take<__nv_bfloat16>(plane * terms(a->dtype));
+    *to = Planes{dst, terms(a->dtype) == 2 ? plane : 0, a->seqlen * heads * dp, int64_t(heads) * dp, dp};
+}
+
 static void plan_pack(const ascan_delta *a, const void *src, const int64_t *strides, int heads, int d, Planes *to, Bump &bump,
                       PackJob *jobs, int *n) {
     if (is_plane(a, src, strides, heads, d)) {
         *to = user_plane(src, strides);
         return;
     }
-    const int dp = round_up8(d);
-    const int64_t plane = a->batch * a->seqlen * heads * dp;
-    __nv_bfloat16 *dst = bump.take<__nv_bfloat16>(plane * terms(a->dtype));
-    *to = Planes{dst, terms(a->dtype) == 2 ? plane : 0, a->seqlen * heads * dp, int64_t(heads) * dp, dp};
-    jobs[(*n)++] = PackJob{src, strides, heads, d, dp, to, plane};
+    take_copy(a, heads, d, to, bump);
+    jobs[(*n)++] = PackJob{src, strides, heads, d, round_up8(d), to, a->batch * a->seqlen * heads * round_up8(d)};
 }
 
 static int run_packs(const ascan_delta *a, const PackJob *jobs, int n, cudaStream_t st) {
@@ -102,8 +106,7 @@ static void take_chunks(DeltaParams &p, Bump &bump) {
     p.P = bump.take<__nv_bfloat16>(each * 2 * 4096);
 }
 
-// keep: what the backward reads again comes first, so that the rest of the layout does not matter to it
-static void fill(const ascan_delta *a, DeltaParams &p, Bump &bump, bool keep, PackJob *jobs, int *n_jobs) {
+static void fill(const ascan_delta *a, DeltaParams &p) {
     p.batch = a->batch;
     p.T = a->seqlen;
     p.packed = a->n_seqs > 0;
@@ -129,9 +132,12 @@ static void fill(const ascan_delta *a, DeltaParams &p, Bump &bump, bool keep, Pa
         p.b_s[i] = a->betas_stride[i];
     }
     p.s0 = a->initial_state;
-    plan_pack(a, a->queries, a->queries_stride, a->heads_k, a->k_dim, &p.q, bump, jobs, n_jobs);
-    plan_pack(a, a->keys, a->keys_stride, a->heads_k, a->k_dim, &p.k, bump, jobs, n_jobs);
-    plan_pack(a, a->values, a->values_stride, a->heads, a->v_dim, &p.v, bump, jobs, n_jobs);
+    p.status = a->status;
+}
+
+// What the backward reads again comes first, at places that only sizes and types decide: the inputs may come to the backward
+// with other strides, and then other ones of them are planes of their own.
+static void take_kept(const ascan_delta *a, DeltaParams &p, Bump &bump, bool keep) {
     const int64_t each = int64_t(p.slots) * p.H;
     p.sc = bump.take<float>(each * SC_ARRAYS * 64);
     if (keep) {
@@ -139,7 +145,32 @@ static void fill(const ascan_delta *a, DeltaParams &p, Bump &bump, bool keep, Pa
         p.S = bump.take<__nv_bfloat16>(each * nt * p.Vp * kp);
         p.e = bump.take<__nv_bfloat16>(each * 2 * 64 * p.Vp);
     }
-    p.status = a->status;
+}
+
+struct Input {
+    const void *src;
+    const int64_t *strides;
+    int heads, d;
+    Planes *to;
+};
+static void list_inputs(const ascan_delta *a, DeltaParams &p, Input (&in)[3]) {
+    in[0] = Input{a->queries, a->queries_stride, a->heads_k, a->k_dim, &p.q};
+    in[1] = Input{a->keys, a->keys_stride, a->heads_k, a->k_dim, &p.k};
+    in[2] = Input{a->values, a->values_stride, a->heads, a->v_dim, &p.v};
+}
+static void plan_inputs(const ascan_delta *a, DeltaParams &p, Bump &bump, PackJob *jobs, int *n) {
+    Input in[3];
+    list_inputs(a, p, in);
+    for (const Input &x : in) plan_pack(a, x.src, x.strides, x.heads, x.d, x.to, bump, jobs, n);
+}
+// The backward's: copies that the forward has left behind what it kept, new ones of what it read as it was and is no plane now.
+static void plan_inputs_again(const ascan_delta *a, DeltaParams &p, Bump &kept, Bump &bump, PackJob *jobs, int *n) {
+    Input in[3];
+    list_inputs(a, p, in);
+    for (int i = 0; i < 3; ++i) {
+        if (a->kept_packed >> i & 1) take_copy(a, in[i].heads, in[i].d, in[i].to, kept);
+        else plan_pack(a, in[i].src, in[i].strides, in[i].heads, in[i].d, in[i].to, bump, jobs, n);
+    }
 }
 
 static bool tensor_core_path(const ascan_delta *a) { return a->dtype == ASCAN_BF16; }
@@ -479,7 +510,9 @@ size_t ascan_delta_forward_bytes(const ascan_delta *a, int keep) {
     Bump bump{nullptr};
     PackJob jobs[4];
     int n = 0;
-    fill(a, p, bump, keep != 0, jobs, &n);
+    fill(a, p);
+    take_kept(a, p, bump, keep != 0);
+    plan_inputs(a, p, bump, jobs, &n);
     if (!tensor_core_path(a)) take_chunks(p, bump);
     return bump.used + 256;
 }
@@ -490,9 +523,20 @@ size_t ascan_delta_backward_bytes(const ascan_delta *a, const void *d_out, const
     Bump bump{nullptr}, none{nullptr};
     PackJob jobs[8];
     int n = 0;
-    fill(a, p, none, true, jobs, &n);
+    fill(a, p);
     fill_back(a, p, bump, d_out, d_out_stride, jobs, &n);
+    plan_inputs_again(a, p, none, bump, jobs, &n);
     return bump.used + 256;
+}
+
+int ascan_delta_packed(const ascan_delta *a) {
+    if (check_shape(a) != ASCAN_OK) return 0;
+    DeltaParams p = {};
+    Input in[3];
+    list_inputs(a, p, in);
+    int packed = 0;
+    for (int i = 0; i < 3; ++i) packed |= is_plane(a, in[i].src, in[i].strides, in[i].heads, in[i].d) ? 0 : 1 << i;
+    return packed;
 }
 
 static int check_pointers(const ascan_delta *a) {
@@ -513,7 +557,9 @@ int ascan_delta_forward(const ascan_delta *a, void *out, float *final_state, int
     Bump bump{static_cast<unsigned char *>(ws)};
     PackJob jobs[4];
     int n = 0;
-    fill(a, p, bump, keep != 0, jobs, &n);
+    fill(a, p);
+    take_kept(a, p, bump, keep != 0);
+    plan_inputs(a, p, bump, jobs, &n);
     if (!tensor_core_path(a)) take_chunks(p, bump);
     p.out = out;
     p.s1 = final_state;
@@ -532,7 +578,7 @@ int ascan_delta_backward(const ascan_delta *a, const void *d_out, const int64_t 
     if (a->batch == 0) return ASCAN_OK;
     if (!d_out_stride) return ASCAN_ERR_INVALID_ARG;
     if (a->seqlen > 0 && !(d_out && d_queries && d_keys && d_values && d_log_gates && d_betas)) return ASCAN_ERR_INVALID_ARG;
-    if (!kept || (reinterpret_cast<uintptr_t>(kept) & 255) || kept_bytes < ascan_delta_forward_bytes(a, 1)) return ASCAN_ERR_WORKSPACE;
+    if (!kept || (reinterpret_cast<uintptr_t>(kept) & 255)) return ASCAN_ERR_WORKSPACE;
     if (!ws || (reinterpret_cast<uintptr_t>(ws) & 255) || ws_bytes < ascan_delta_backward_bytes(a, d_out, d_out_stride))
         return ASCAN_ERR_WORKSPACE;
     int sms = 0;
@@ -541,9 +587,11 @@ int ascan_delta_backward(const ascan_delta *a, const void *d_out, const int64_t 
     Bump saved{static_cast<unsigned char *>(kept)}, bump{static_cast<unsigned char *>(ws)};
     PackJob jobs[8];
     int n = 0;
-    fill(a, p, saved, true, jobs, &n);
-    n = 0;                                     // the inputs' planes are in `kept`
+    fill(a, p);
+    take_kept(a, p, saved, true);
     fill_back(a, p, bump, d_out, d_out_stride, jobs, &n);
+    plan_inputs_again(a, p, saved, bump, jobs, &n);
+    if (kept_bytes < saved.used) return ASCAN_ERR_WORKSPACE;
     p.d_s1 = d_final_state;
     p.d_s0 = d_initial_state;
     p.d_q = d_queries;

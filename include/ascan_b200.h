@@ -366,6 +366,7 @@ typedef struct {
     const float *initial_state;
     const void *seq_starts;
     int32_t n_seqs, seq_starts_64;                 /* n_seqs == 0: not packed                 */
+    int32_t kept_packed;                           /* read by the backward alone: see ascan_delta_packed */
     int *status;                                   /* nullable, device-accessible host memory: a kernel whose bounded
                                                       wait expired stores 1; its results are then invalid */
 } ascan_delta;
@@ -376,16 +377,24 @@ typedef struct {
  */
 size_t ascan_delta_forward_bytes(const ascan_delta *args, int keep);
 
+/*
+ * Which inputs the forward with these arguments packs, and with keep != 0 leaves behind what it keeps: 1 for queries,
+ * 2 for keys, 4 for values (those of float and half, and bf16 ones with strides or addresses that tiles cannot be
+ * copied from).  The backward gets that number of the forward's arguments as kept_packed and then reads those
+ * copies.  Where it is 0 the backward packs again what it needs.
+ */
+int ascan_delta_packed(const ascan_delta *args);
+
 /* out: dense (batch, seqlen, heads, v_dim) of dtype.  ws: 256-byte aligned, not initialised, one per call in flight. */
 int ascan_delta_forward(const ascan_delta *args, void *out, float *final_state, int keep,
                         void *ws, size_t ws_bytes, void *stream);
 
-/* Scratch bytes of ascan_delta_backward for this gradient of out. */
+/* Scratch bytes of ascan_delta_backward for these arguments (kept_packed among them) and this gradient of out. */
 size_t ascan_delta_backward_bytes(const ascan_delta *args, const void *d_out, const int64_t *d_out_stride);
 
 /*
- * Gradients of ascan_delta_forward, dense, of their inputs' shapes and types.  args and kept are those of a forward
- * with keep != 0.  d_final_state may be NULL (zero), d_initial_state may be NULL (not wanted).  Heads that share a key
+ * Gradients of ascan_delta_forward, dense, of their inputs' shapes and types.  kept is the scratch of a forward with
+ * keep != 0, args hold the same sizes, types, values and sequences; addresses and strides may be others.  d_final_state may be NULL (zero), d_initial_state may be NULL (not wanted).  Heads that share a key
  * head are summed in a fixed order.
  */
 int ascan_delta_backward(const ascan_delta *args, const void *d_out, const int64_t *d_out_stride,
