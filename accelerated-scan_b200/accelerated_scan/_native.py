@@ -13,6 +13,7 @@ import os
 import struct
 
 import torch
+from torch.autograd import forward_ad
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libascan_b200.so")
@@ -230,6 +231,13 @@ def _raw_stream(device) -> int:
 def _rows_T(t):
     T = t.shape[-1]
     return (t.numel() // T if T else 0), T
+
+
+def refuse_tangents(what, *tensors):
+    """Calls that do not go through an autograd function, which would raise this itself, must not drop a tangent."""
+    if forward_ad._current_level >= 0 and any([isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None
+                                               for t in tensors]):
+        raise NotImplementedError(f"{what} has no forward-mode derivative")
 
 
 _NULL_GUARD = contextlib.nullcontext()

@@ -23,7 +23,7 @@ _DTYPES = (torch.float32, torch.bfloat16, torch.float16)
 MAX_KEY_DIM, MAX_VALUE_DIM = 128, 1024
 
 
-def _check_inputs(lead, queries, keys, values, log_gates, betas):
+def _check_inputs(lead, queries, keys, values, log_gates, betas, state):
     """lead: names of the dimensions before the heads."""
     n = len(lead)
     assert queries.dim() == n + 2, f"queries must have shape ({', '.join(lead)}, key heads, K)"
@@ -31,6 +31,7 @@ def _check_inputs(lead, queries, keys, values, log_gates, betas):
     assert values.dim() == n + 2 and values.shape[:n] == queries.shape[:n], f"values must have shape ({', '.join(lead)}, heads, V)"
     heads_k, K = queries.shape[n:]
     heads, V = values.shape[n:]
+    _native.refuse_tangents("the gated delta rule", queries, keys, values, log_gates, betas, state)
     assert heads_k > 0 and heads > 0 and heads % heads_k == 0, "the value heads must be a multiple of the key heads"
     assert log_gates.shape == values.shape[:n + 1], f"log_gates must have shape ({', '.join(lead)}, heads)"
     assert betas.shape == values.shape[:n + 1], f"betas must have shape ({', '.join(lead)}, heads)"
@@ -120,11 +121,13 @@ def scan(queries, keys, values, log_gates, betas, initial_state=None, scale=None
 
     Strides are free but for the last dimension of queries, keys and values, which has to be dense (it is copied if not).
 
+    Differentiable in reverse mode, once; a forward-mode tangent is refused.
+
     Returns:
         out (torch.Tensor): (B, T, heads, V) in the dtype of values
         final_state (torch.Tensor): (sequences, heads, K, V) float32, to hand to the next call
     """
-    _check_inputs(("B", "T"), queries, keys, values, log_gates, betas)
+    _check_inputs(("B", "T"), queries, keys, values, log_gates, betas, initial_state)
     B, _, _, K = queries.shape
     H, V = values.shape[2:]
     n = B
@@ -165,7 +168,7 @@ def step(queries, keys, values, log_gates, betas, state, slots=None, scale=None)
     Returns:
         out (torch.Tensor): (B, heads, V).  Not differentiable; use `scan` to train.
     """
-    _check_inputs(("B",), queries, keys, values, log_gates, betas)
+    _check_inputs(("B",), queries, keys, values, log_gates, betas, state)
     B, _, K = queries.shape
     H, V = values.shape[1:]
     assert state.dim() == 4 and state.shape[1:] == (H, K, V), "state must have shape (pool, heads, K, V)"

@@ -88,6 +88,8 @@ def residual_norm(block_out, residual=None, *, post_weight=None, gate=None, scal
             per channel.
         activation (str, optional): "sigmoid", "silu" (gate * sigmoid(gate)), or None for the gate as it is.
 
+    Differentiable in reverse mode, once; a forward-mode tangent is refused.
+
     Returns:
         hidden, or (hidden, normed) where pre_weight is given; normed is computed from hidden before its rounding.
     """
@@ -110,6 +112,7 @@ def residual_norm(block_out, residual=None, *, post_weight=None, gate=None, scal
         assert w.shape == (D,), "weights and a scale per channel must have shape (D,)"
         if w.dtype not in (x.dtype, torch.float32) or w.dtype != vectors[0].dtype:
             raise RuntimeError("weights and scale must all be of block_out's dtype or all float32")
+    _native.refuse_tangents("residual_norm", x, residual, gate, *vectors)
     if not x.is_cuda:
         raise RuntimeError("tensors must be CUDA tensors")
     for t in (residual, gate, *vectors):
