@@ -195,4 +195,5 @@ def step(queries, keys, values, log_gates, betas, state, slots=None, scale=None)
     if B:
         queries, keys, values = _dense_last(queries), _dense_last(keys), _dense_last(values)
         _native.delta_step(queries, keys, values, log_gates, betas, out, state, slots, K ** -0.5 if scale is None else float(scale))
+        torch.autograd.graph.increment_version(state)       # written through its pointer: whoever saved it for a backward hears of it
     return out
