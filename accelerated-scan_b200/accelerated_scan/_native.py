@@ -591,8 +591,10 @@ def delta_step(queries, keys, values, log_gates, betas, out, state, slots, scale
         B, heads_k, heads, K, V, DTYPE_CODE[queries.dtype], DTYPE_CODE[log_gates.dtype], DTYPE_CODE[betas.dtype], scale,
         _sink(queries.device))
     device = queries.device
+    pool = state.shape[0]
+    slot_stride = state.stride(0) if pool > 1 else heads * K * V         # torch leaves the stride of one element open
     with _device_guard(device):
-        rc = lib.ascan_delta_step(args, out.data_ptr(), state.data_ptr(), state.shape[0], state.stride(0), _ptr(slots),
+        rc = lib.ascan_delta_step(args, out.data_ptr(), state.data_ptr(), pool, slot_stride, _ptr(slots),
                                   slots is not None and slots.dtype == torch.int64, _raw_stream(device))
     _launched(rc, "ascan_delta_step")
 

@@ -44,3 +44,25 @@ def test_no_rows_change_nothing(cuda_device):
     before = pool._version
     delta.step(*args, pool)
     assert pool._version == before
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("view", [lambda t: t.view(2, 1, 16, 16).transpose(0, 1), lambda t: t.as_strided((1, 2, 16, 16), (0, 256, 16, 1)),
+                                  lambda t: t.as_strided((1, 2, 16, 16), (7, 256, 16, 1))])
+@pytest.mark.parametrize("slots", [False, True])
+def test_a_pool_of_one_state_has_any_first_stride(cuda_device, view, slots):
+    args = token_inputs(4, 1, 1, 2, 16, 16, torch.float32, cuda_device)
+    slots = torch.zeros(1, dtype=torch.int64, device=cuda_device) if slots else None
+    plain = torch.randn(1, 2, 16, 16, device=cuda_device)
+    odd = view(plain.clone())
+    assert odd.shape == plain.shape and odd.stride(0) < 512
+    want = delta.step(*args, plain, slots)
+    assert torch.equal(delta.step(*args, odd, slots), want) and torch.equal(odd, plain)
+
+
+@pytest.mark.gpu
+def test_a_pool_without_states(cuda_device):
+    """Every slot lies behind it, or is a padded row."""
+    args = token_inputs(5, 2, 1, 2, 16, 16, torch.float32, cuda_device)
+    out = delta.step(*args, torch.empty(0, 2, 16, 16, device=cuda_device), torch.tensor([0, -1], device=cuda_device))
+    assert torch.isnan(out[0]).all() and (out[1] == 0).all()
