@@ -259,24 +259,34 @@ struct RowSum {
 };
 
 // The gates' values in place of the gates, and their slopes: s c with c = 1 or z, and s ((1 - s) c + 0 or 1).
-template <bool SLOPE, int E>
+// s = 1 / (1 + 2^t), t = -z log2 e, by the two approximations (2^-22 and 2^-23 of the result): two slow instructions an element,
+// where the exact exponential and division took half of a kernel's time.  Past |z| = 88 it is 0 and 1.  1 - s, which would cancel
+// where a gate is open, is s 2^t.
+// t is off by its rounding and that of log2 e, |t| 2^-23, and 2^t by as much of itself: 2^-16 at |z| = 80.  For results of 16 bits
+// that is little beside their own 2^-9 and 2^-12.  FINE, for fp32: what t is off goes onto 2^t as a factor, and the gate is within
+// 10 2^-24, the slope within 24 2^-24 of its terms.
+template <bool SLOPE, bool FINE, int E>
 __device__ __forceinline__ void open_gates(float (&z)[E], float (&slope)[E], int act) {
     if (act == ACT_NONE) {
 #pragma unroll
         for (int i = 0; i < E; ++i) slope[i] = 1.f;
         return;
     }
+    constexpr float LOG2E = 1.4426950408889634f, LOG2E_LO = 1.92596299112661746e-8f, LN2 = 0.693147180559945309f;
     const bool silu = act == ACT_SILU;
     const float one = silu ? 1.f : 0.f;
 #pragma unroll
     for (int i = 0; i < E; ++i) {
-        // 1 / (1 + 2^(-z log2 e)), each part good to a few 2^-24: two slow instructions an element, where the exact
-        // exponential and division took half of a kernel's time.  Past |z| = 88 it is 0 and 1.
+        const float t = z[i] * -LOG2E;
         float e, s;
-        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(z[i] * -1.4426950408889634f));
+        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
+        if (FINE) {
+            const float off = fmaf(z[i], -LOG2E_LO, fmaf(z[i], -LOG2E, -t));
+            e = fabsf(z[i]) < 88.f ? fmaf(e, LN2 * off, e) : e;              // beyond, 2^t is infinite or nothing beside 1
+        }
         asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(s) : "f"(1.f + e));
         const float c = silu ? z[i] : 1.f;
-        if (SLOPE) slope[i] = s * fmaf(1.f - s, c, one);
+        if (SLOPE) slope[i] = s * fmaf(s * fminf(e, 3.402823466e38f), c, one);
         z[i] = s * c;
     }
 }
@@ -331,7 +341,7 @@ __global__ void __launch_bounds__(E == 8 ? 256 : 512, E == 8 ? 3 : 1) norm_forwa
         }
         if (p.gate) {
             float none[E];
-            open_gates<false>(z, none, p.act);
+            open_gates<false, sizeof(T) == 4>(z, none, p.act);
 #pragma unroll
             for (int i = 0; i < E; ++i) r[i] += w[i] * (z[i] * (x[i] * rx));
         } else {
@@ -432,7 +442,7 @@ __global__ void __launch_bounds__(FORM == LEAN ? 256 : FORM == WIDE_ROWS ? NORM_
         }
         float slope[EPT];
         if (p.gate) {
-            open_gates<true>(z, slope, p.act);                            // from here on the gate's value
+            open_gates<true, sizeof(T) == 4>(z, slope, p.act);                            // from here on the gate's value
         } else {
 #pragma unroll
             for (int i = 0; i < EPT; ++i) {
