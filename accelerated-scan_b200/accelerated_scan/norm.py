@@ -63,6 +63,9 @@ class ResidualNorm(torch.autograd.Function):
         if d_hidden is None and d_normed is None:
             return (None,) * 8
         D = x.shape[-1]
+        # saved-tensor hooks may hand back equal tensors that lie in memory in another way
+        x, residual, gate = _rows(x, D), _rows(residual, D), _rows(gate, D)
+        post_weight, scale, pre_weight = (None if w is None else w.contiguous() for w in (post_weight, scale, pre_weight))
         need = ctx.needs_input_grad
         new = lambda t: torch.empty(ctx.shape, dtype=t.dtype, device=t.device)
         d_x = new(x)
