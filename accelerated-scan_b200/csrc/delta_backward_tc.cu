@@ -136,7 +136,7 @@ __device__ __forceinline__ void back_sweep(const DeltaParams &p, const TcMaps &m
             }
             const int64_t left = sq.len - int64_t(c) * 64;
             const bool by_copy = maps.store && (left >= 64 || sq.t0 + sq.len == p.T);        // as in the forward sweep
-            if (by_copy) fence_async_proxy();
+            fence_async_proxy();
             group_sync<1, 256>();
             const uint32_t tile = base + stage * L::STAGE + L::KQ_BYTES;
             if (by_copy) {

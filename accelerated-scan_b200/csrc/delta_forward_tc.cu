@@ -167,7 +167,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) delta_sweep_tc_kernel(const __g
             const int64_t left = sq.len - int64_t(c) * 64;
             // One copy takes the tile to memory; it leaves out rows behind the array, but not those of a next sequence.
             const bool by_copy = maps.store && (left >= 64 || sq.t0 + sq.len == p.T);
-            if (by_copy) fence_async_proxy();
+            fence_async_proxy();                  // before this copy reads the tile, or the next chunk's copies write over it
             group_sync<1, 256>();
             if (by_copy) {
                 if (tid == 0) {
