@@ -121,6 +121,17 @@ def scan(queries, keys, values, log_gates, betas, initial_state=None, scale=None
 
     Strides are free but for the last dimension of queries, keys and values, which has to be dense (it is copied if not).
 
+    Precision, as 2-norm of the error over that of the result.  The products are taken on bf16 tensor cores with fp32 sums, and
+    operands that are not bf16 as two terms, 2^-16 of each: states and fp32 results are 5e-6 to 1e-5 off (elementary fp32
+    operations: 2e-7), fp16 results little more than their rounding, bf16 ones likewise but for `out`, which reads the
+    state and the weights within a chunk in one term: 2.4e-3, of which 1.7e-3 is its own rounding.  That is for unit keys and
+    rates up to 1.  A rate of 2 reflects the state along its key; the same key over and over, undecayed, then lets the errors
+    of a chunk add up (states 4e-3 off from bf16 inputs, 8e-4 from others).
+
+    Log gates above zero let the state grow; where they rise by more than 88 in all, fp32 overflows.  What is not finite makes
+    NaN of its whole chunk of 64 tokens, the ones before it too, and of what follows, also behind a beta or a gate of zero:
+    padding within a sequence has to hold finite numbers.  Tokens outside of all sequences may hold anything.
+
     Differentiable in reverse mode, once; a forward-mode tangent is refused.
 
     Returns:
