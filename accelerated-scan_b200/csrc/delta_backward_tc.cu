@@ -155,6 +155,7 @@ __device__ __forceinline__ void back_sweep(const DeltaParams &p, const TcMaps &m
                         static_cast<bf16 *>(p.d_v)[((row0 + t) * p.H + h) * p.V + v0 + u] = *reinterpret_cast<const bf16 *>(
                             tp + (u >> 6) * 8192 + t * 128 + (((u >> 3 & 7) ^ (t & 7)) << 4) + (u & 7) * 2);
                 }
+                give_back_reads();
             }
             const float gam_c = sc[SC_GAM * 64 + 63 - part * 32];
             const f2 gam_c2 = two(gam_c, gam_c);

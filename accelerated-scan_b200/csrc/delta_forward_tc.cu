@@ -185,6 +185,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) delta_sweep_tc_kernel(const __g
                         static_cast<bf16 *>(p.out)[((row0 + t) * p.H + h) * p.V + col] =
                             *reinterpret_cast<const bf16 *>(ot + t * 256 + (i & 127) * 2);
                 }
+                give_back_reads();
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(k.bar(B_FREE + stage));

@@ -144,8 +144,7 @@ __device__ __forceinline__ void chunk_gradients(const DeltaParams &p, const Grad
                     if ((lane & 15) == 0) direct[t >> 4] = ((ok >> (lane & 16)) & 0xffffu) != 0xffffu;
                 }
                 const float gam_c = sc[SC_GAM * 64 + 63];
-                // <S0, dS1>: 16 products a thread and slab, by plain loads (as a diagonal of warp products, beside the tcgen05 products
-                // that read the same slab, it differed from run to run)
+                // <S0, dS1>: 16 products a thread and slab, by plain loads (480 us a launch; as a diagonal of warp products 489)
                 float dot_s = 0.f;
 #pragma unroll 1
                 for (int s = 0; s < slabs; ++s, ++n_slab) {
@@ -159,6 +158,7 @@ __device__ __forceinline__ void chunk_gradients(const DeltaParams &p, const Grad
 #pragma unroll
                         for (int j = 0; j < 4; ++j) dot_s += low_half(xs[j]) * low_half(ys[j]) + high_half(xs[j]) * high_half(ys[j]);
                     }
+                    give_back_reads();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(bar(G_SLAB_FREE + (n_slab & 1)));
                 }
@@ -312,6 +312,8 @@ __device__ __forceinline__ void chunk_gradients(const DeltaParams &p, const Grad
                     }
                 }
             }
+            give_back_reads();
+            __syncwarp();
             if (lane == 0) mbar_arrive(bar(G_KQ_FREE));
             ++n_item;
             // dQ and dK of the key head (the barrier before the sums has seen all their columns)

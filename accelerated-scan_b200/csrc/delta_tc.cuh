@@ -71,6 +71,10 @@ __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::
 __device__ __forceinline__ void tc_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void fence_async_proxy() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+// A thread's reads of a tile have ended, before it says that the next copy may write over it.  An arrival alone does not wait for
+// loads of the generic proxy that are still queued behind the tensor cores' operands: sums of such reads came out of the next
+// tile's values in most runs, d_log_gates off by up to a sixth of the largest, until this stood before the arrival.
+__device__ __forceinline__ void give_back_reads() { fence_async_proxy(); }
 __device__ __forceinline__ void tc_commit(uint32_t bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" :: "r"(bar) : "memory");
 }

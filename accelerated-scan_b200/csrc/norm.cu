@@ -201,6 +201,7 @@ struct RowRing {
         }
     }
     __device__ __forceinline__ void release() {          // everybody has read: ask for the rows that come here next
+        give_back_reads();
         __syncthreads();
         if (threadIdx.x == 0) issue(stage);
         if (++stage == p.stages) {
