@@ -503,8 +503,9 @@ def backward_time_sharded(gates, states, grad_out, d_gates, d_tokens, rank: int,
     _finish(rc, "ascan_backward_time_sharded", ws, stream)
 
 
-# Gated delta rule and norms.  Their kernels wait for nothing, keep nothing between calls and take ordinary tensors of
-# torch's allocator as scratch, so calls on different streams and captured graphs never share any.
+# Gated delta rule and norms.  Their kernels keep nothing between calls and take ordinary tensors of torch's allocator as
+# scratch, so calls on different streams and captured graphs never share any.  They wait for copies and CTAs of their own
+# launch only; a wait that expires is reported through a word of pinned host memory.
 
 def _launched(rc, what):
     global launch_count

@@ -14,8 +14,9 @@
 // What bounds it is the chain of a chunk, about 8000 clocks: five products, each followed by a conversion of the result into
 // the next one's operand (6500 clocks of the 256 threads' work and waits), and beside it the preparation of M, 11000 to
 // 13000 clocks a chunk over two groups.  Sequences times heads give the parallelism, so memory waits: 4 x 16384 tokens, 32
-// heads of 128 x 128 take 1078 us (1.6 GB, 1.5 TB/s; the same on warp matrix instructions 3344 us), nine packed prompts of
-// 8192 tokens 211 us, 4 x 4096 tokens of 16 heads, with what the backward needs, 383 us.
+// heads of 128 x 128 take 1075 us (1.6 GB, 1.5 TB/s; the same on warp matrix instructions 3344 us), nine packed prompts of
+// 8192 tokens in all 165 to 300 us (the longest has 1830 to 4000, and its turn comes first or later), 4 x 4096 tokens of 16
+// heads 267 us, with what the backward needs 383 us.
 #include "delta_tc_roles.cuh"
 
 namespace ascan {

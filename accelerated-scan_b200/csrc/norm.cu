@@ -10,8 +10,10 @@
 // its rows.  Sums of the weights' gradients over CTAs are a second launch, in a fixed order.
 //
 // Measured, bf16: 32768 rows of 4096 with all parts, forward, 276 us (1.34 GB, 4.9 TB/s; 6.55 are a plain copy's); 262144
-// heads of 128 with a gate, forward 52 us and backward 85 us (201 and 335 MB, 3.9 TB/s).  What is missing is issue slots:
-// 2.3 - 2.7 instructions a clock, of which conversions, gates and the rows' reductions are most.
+// heads of 128 with a gate, forward 52 us and backward 85 us (201 and 335 MB, 3.9 TB/s).  Backward with all parts, 2.15 GB each:
+// 32768 rows of 4096 823 us, 16384 of 8192 1716 us; in fp32, 16384 of 4096, 471 us.  What is missing is issue slots and warps to
+// hide latencies: 2.7 of 4 instructions a clock at 35 % of the warps (rows of 128), 2.0 to 2.2 at 25 % (long rows), where fixed
+// latencies, shared loads and barriers stall about equally; conversions, gates and the rows' reductions are most of the work.
 #include <atomic>
 
 #include "delta_tc.cuh"
@@ -367,7 +369,9 @@ __global__ void __launch_bounds__(E == 8 ? 256 : 512, E == 8 ? 3 : 1) norm_forwa
 // With x' the normed x, z the gate's value and dh the gradient of h: sum over rows of dh z x' is the gradient of post_weight but
 // for the factor scale, and that of scale but for the factor post_weight, so one sum serves both, and one product of the two
 // weights the rest.  WIDE: rows whose threads have only 64 registers each.  The weights are read where they are used (from the L1 cache) and
-// their gradients are summed in shared memory, by the thread that owns the element.
+// their gradients are summed in shared memory, by the thread that owns the element.  It spills 240 to 400 bytes a thread all the
+// same, and beside the sums no ring of 16-bit rows of 8192 fits: 16384 x 8192 waits for memory (1.3 TB/s), twice the time
+// that the same elements take in rows of 4096.
 template <class T, bool ALIGNED, int FORM, bool RING>
 __global__ void __launch_bounds__(FORM == LEAN ? 256 : FORM == WIDE_ROWS ? NORM_THREADS : NORM_NARROW, FORM == LEAN ? 3 : 1) norm_backward_kernel(const __grid_constant__ NormParams p) {
     extern __shared__ __align__(128) unsigned char dynamic[];
